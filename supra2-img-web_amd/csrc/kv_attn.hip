@@ -1,0 +1,528 @@
+// Attention over the 8-bit key/value cache (include/supra_kv.h).
+//
+// One workgroup takes 32 rows (tokens x query heads of one key head: t * G + g) and a share of the sequence's pages;
+// its four waves take the pages in turn and their results are merged at the end. A page is 32 keys, the tile of a
+// 32x32x16 matrix instruction: S^T = K Q^T leaves a row's scores in the lanes l and l + 32 (register 4 g + r of half
+// h: key 8 g + 4 h + r), which is the operand order of O^T += V^T P^T, and the order V's codes have in the cache. So
+// neither K, V nor P changes lanes, and a page's K and V come as 16-byte loads of 1 KiB per wave.
+//
+// Numbers. K and V codes are exact in float16 (v_cvt_scalef32_pk_f16_fp8), V's with its page's scale relative to the
+// largest one so far (2^m_v; a growing one rescales the sums like the running maximum). Q is brought to float16 by a
+// power of two of each row, its largest magnitude in [2^14, 2^15): float16 and bfloat16 rows in one term, exactly down
+// to 2^-28 of the row's largest element; float32 rows in two terms, 22 bits of each element. The probabilities, at
+// 2^kPBias for the running maximum, are one float16 term (11 bits: half a step of it is a sixteenth of a bfloat16
+// output's, and half a float16 one's, before the sum averages them) or two for float32 rows. Sums, maxima and products
+// are float32.
+//
+// V relative to the largest scale: codes times 2^(e - m_v + 6) stay exact for pages down to 2^-21 of the largest
+// page of the head, and below that are off by at most 2^-40 of its largest value.
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+
+#include "common.h"
+#include "kv_check.h"
+#include "kv_layout.h"
+#include "row_types.h"
+
+namespace sa {
+
+namespace {
+
+constexpr int kCUs = 256;      // of an MI355X: what the splits are planned for
+constexpr int kRows = 32;      // rows of a workgroup
+constexpr int kPBias = 10;     // log2 of a probability's scale at the running maximum
+constexpr float kLazy = 4.f;   // the maximum moves when a score passes it by more than this (log2): P stays below 2^14
+constexpr int kVBias = 6;      // log2 of V's scale at the largest page
+
+struct KvAttnParams {
+  sa_kv_cache c;
+  sa_kv_seqs s;
+  const char* q;  // offset included; strides in bytes
+  char* o;
+  int64_t ldq, ldo;
+  float* ws;      // records of the splits, or null
+  float scale_log2;
+  int H, G;       // query heads, and of one key head
+  int causal;
+  int groups;     // row groups of a sequence (of max_rows)
+  int splits;
+  int aligned_q, aligned_o;  // rows of 16-byte aligned heads
+};
+
+template <typename T>
+constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+
+__device__ __forceinline__ f16x8 half8(uint32_t a, uint32_t b, float scale) {
+  const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false), x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true),
+              x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false), x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true);
+  return f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+
+__device__ __forceinline__ f16x8 round8(const float* x) {
+  f16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const f16x2 p = __builtin_convertvector((f32x2{x[i], x[i + 1]}), f16x2);
+    y[i] = p[0], y[i + 1] = p[1];
+  }
+  return y;
+}
+
+// hi[0..NT): x in NT float16 terms.
+template <int NT>
+__device__ __forceinline__ void split8(const float* x, f16x8 (&y)[NT]) {
+  y[0] = round8(x);
+  if constexpr (NT == 2) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] - (float)y[0][i];
+    y[1] = round8(r);
+  }
+}
+
+__device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// What a workgroup works on.
+struct Work {
+  KvSeq q;
+  int b, hk, row0, rows;  // packed rows [row0, row0 + 32) of rows * G
+  int blocks;             // pages that any of its rows attends to
+};
+
+__device__ __forceinline__ bool kv_work(const KvAttnParams& a, int group, int hk, int b, Work* w) {
+  w->q = kv_seq(a.s, b);
+  w->b = b;
+  w->hk = hk;
+  w->row0 = group * kRows;
+  w->rows = w->q.rows * a.G;
+  if (w->row0 >= w->rows) return false;
+  int keys = w->q.len;
+  if (a.causal) {
+    const int t = (min(w->row0 + kRows, w->rows) - 1) / a.G;  // the last row's token
+    keys = max(0, min(keys, w->q.first + t + 1));
+  }
+  w->blocks = (keys + kKvBlock - 1) / kKvBlock;
+  return true;
+}
+
+// Q's operand for one 32-row group: lane (row = lane & 31, half): elements 32c + 16 half .. + 16 of each chunk c.
+template <typename T, int D>
+struct QTile {
+  f16x8 t[D / 32][2][kTerms<T>];
+  int exponent;  // the row's elements are 2^exponent times the operand's
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int lane, QTile<T, D>& q) {
+  const int r = w.row0 + (lane & 31), half = lane >> 5;
+  const bool on = r < w.rows;
+  const T* p = nullptr;
+  if (on) p = reinterpret_cast<const T*>(a.q + (int64_t)(w.q.row0 + r / a.G) * a.ldq) + (int64_t)(w.hk * a.G + r % a.G) * D + 16 * half;
+  float x[D / 32][16];
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[c][i] = 0.f;
+    if (on) {
+      if (a.aligned_q) load_row<T, 16, true>(p + 32 * c, x[c]);
+      else load_row<T, 16, false>(p + 32 * c, x[c]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[c][i]) & 0x7fffffffu);
+  }
+  auto sw = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max(sw[0], sw[1]);
+  // factor 2^(14 - exponent of the largest): an infinity or NaN among them gives NaN scores, as in float32
+  const int f = min(127 + 14 + 127 - (int)(m >> 23), 253);
+  q.exponent = 127 - f;
+  const float factor = __uint_as_float((uint32_t)f << 23);
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[c][i] *= factor;
+    split8<kTerms<T>>(x[c], q.t[c][0]);
+    split8<kTerms<T>>(x[c] + 8, q.t[c][1]);
+  }
+}
+
+// The running state of 32 rows in one wave: O^T (chunk c, register 4 g + r of half h: element 32 c + 8 g + 4 h + r of
+// row lane & 31), the maximum (log2 units, one for both halves of a row) and this half's sum.
+template <int D>
+struct State {
+  f32x16 o[D / 32];
+  float m, l;
+  int mv;  // exponent byte of V's reference scale
+};
+
+// Bytes 0x7f and 0xff are NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// One page of 32 keys. kr, vr: its K and V tiles, 16 bytes of each KiB per lane. MASKED: of the page's keys each row
+// attends to the first `limit` (its own).
+template <typename T, int D, bool MASKED>
+__device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const u32x4 (&kr)[D / 32], const u32x4 (&vr)[D / 32], int ke,
+                                     int ve, float scale_log2, int lane, int limit) {
+  constexpr int NT = kTerms<T>;
+  f32x16 s = zero16();
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    const f16x8 k0 = half8(kr[c][0], kr[c][1], 1.f), k1 = half8(kr[c][2], kr[c][3], 1.f);
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t) {
+      s = mfma(k0, q.t[c][0][t], s);
+      s = mfma(k1, q.t[c][1][t], s);
+    }
+  }
+  const float f = ldexpf(scale_log2, q.exponent + ke - 127);
+  const int half = lane >> 5;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] *= f;
+    if constexpr (MASKED) s[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? s[i] : -INFINITY;
+    top = max_nan(top, s[i]);
+  }
+  top = max_with_partner(top);
+  const bool grows = !(top <= st.m + kLazy), v_grows = ve > st.mv;
+  if (__any(grows) || v_grows) {
+    const float m = grows ? max_nan(st.m, top) : st.m;
+    float r = fast_exp2(st.m - m);
+    st.l *= r;
+    if (v_grows) {
+      r *= __uint_as_float(kv_pow2_bits(st.mv - ve));
+      st.mv = ve;
+    }
+    st.m = m;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[c][i] *= r;
+  }
+  float p[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    p[i] = fast_exp2(s[i] - st.m + (float)kPBias);
+    st.l += p[i];
+  }
+  f16x8 p0[NT], p1[NT];
+  split8<NT>(p, p0);
+  split8<NT>(p + 8, p1);
+  const float vs = __uint_as_float((uint32_t)max(ve - st.mv + kVBias + 127, 1) << 23);
+  u32x4 v[D / 32];
+  bool nan_v = false;
+  if constexpr (MASKED) {
+    // A key that a row does not attend to may hold NaN in V, and 0 * NaN is not 0.
+    uint32_t any = 0;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= nan_bytes(vr[c][i]);
+    nan_v = __any(any != 0);
+  }
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    v[c] = vr[c];
+    if (MASKED && nan_v) {
+      // NaN codes leave the tile, and a product of their places with the attended keys says whose sums they turn
+      // into NaN.
+      u32x4 at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t n = nan_bytes(v[c][i]) >> 7, whole = n * 0xffu;
+        v[c][i] &= ~whole;
+        at[i] = n * 0x38u;  // the code of 1
+      }
+      float seen[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) seen[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? 1.f : 0.f;
+      f32x16 hits = zero16();
+      hits = mfma(half8(at[0], at[1], 1.f), round8(seen), hits);
+      hits = mfma(half8(at[2], at[3], 1.f), round8(seen + 8), hits);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[c][i] = hits[i] > 0.f ? NAN : st.o[c][i];
+    }
+    const f16x8 v0 = half8(v[c][0], v[c][1], vs), v1 = half8(v[c][2], v[c][3], vs);
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t) {
+      st.o[c] = mfma(v0, p0[t], st.o[c]);
+      st.o[c] = mfma(v1, p1[t], st.o[c]);
+    }
+  }
+}
+
+// A split's record: 32 rows of D floats, then their 32 log2-sums.
+constexpr int64_t record_floats(int D) { return (int64_t)kRows * (D + 1); }
+
+template <typename T, int D>
+__device__ __forceinline__ void store_o4(const KvAttnParams& a, const Work& w, int row, int d, f32x4 x) {
+  T* p = reinterpret_cast<T*>(a.o + (int64_t)(w.q.row0 + row / a.G) * a.ldo) + (int64_t)(w.hk * a.G + row % a.G) * D + d;
+  const float y[4] = {x[0], x[1], x[2], x[3]};
+  if (a.aligned_o) store_row<T, 4, true>(p, y);
+  else store_row<T, 4, false>(p, y);
+}
+
+constexpr int kSplitWaves = 4;
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kSplitWaves, D * kTerms<T> <= 128 ? 2 : 1) void kv_attn_split_kernel(KvAttnParams a) {
+  constexpr int C = D / 32, PAD = 36;
+  __shared__ __attribute__((aligned(16))) float lo[kSplitWaves][kRows][PAD];
+  __shared__ float lm[kSplitWaves][kRows], ll[kSplitWaves][kRows];
+  __shared__ int lv[kSplitWaves];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int group = id % a.groups;
+  id /= a.groups;
+  Work w;
+  if (!kv_work(a, group, id % a.c.Hkv, id / a.c.Hkv, &w)) return;
+  const int lo_block = (int)((int64_t)w.blocks * split / a.splits), hi_block = (int)((int64_t)w.blocks * (split + 1) / a.splits);
+
+  QTile<T, D> q;
+  load_q<T, D>(a, w, lane, q);
+  State<D> st;
+#pragma unroll
+  for (int c = 0; c < C; ++c) st.o[c] = zero16();
+  st.m = kMaxSeed;
+  st.l = 0.f;
+  st.mv = 0;
+
+  // The row's own limit: keys [0, limit) of the sequence.
+  const int row = w.row0 + (lane & 31);
+  int limit = w.q.len;
+  if (a.causal) limit = min(limit, w.q.first + row / a.G + 1);
+  int least = w.q.len;  // the least of the group's rows
+  if (a.causal) least = min(least, w.q.first + w.row0 / a.G + 1);
+
+  const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
+  const int place = (lane & 31) * 32 + (lane >> 5) * 16;
+  for (int blk = lo_block + wave; blk < hi_block; blk += kSplitWaves) {
+    const int32_t page = table[blk];
+    if (!kv_page_ok(page, a.c.pages)) continue;
+    const int64_t at = kv_tile(page, a.c.Hkv, w.hk, D) + place;
+    u32x4 kr[C], vr[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) kr[c] = *reinterpret_cast<const u32x4*>(a.c.k + at + c * 1024);
+#pragma unroll
+    for (int c = 0; c < C; ++c) vr[c] = *reinterpret_cast<const u32x4*>(a.c.v + at + c * 1024);
+    const int ke = a.c.k_scale[(int64_t)page * a.c.Hkv + w.hk], ve = a.c.v_scale[(int64_t)page * a.c.Hkv + w.hk];
+    if ((blk + 1) * kKvBlock <= least) step<T, D, false>(q, st, kr, vr, ke, ve, a.scale_log2, lane, 0);
+    else step<T, D, true>(q, st, kr, vr, ke, ve, a.scale_log2, lane, limit - blk * kKvBlock);
+  }
+
+  // ---- merge of the waves
+  const float l = sum_with_partner(st.l);
+  if (lane < 32) {
+    lm[wave][lane] = st.m;
+    ll[wave][lane] = l;
+  }
+  if (lane == 0) lv[wave] = st.mv;
+  __syncthreads();
+  const int r = lane & 31, half = lane >> 5;
+  float m = lm[0][r];
+  int mv = lv[0];
+#pragma unroll
+  for (int i = 1; i < kSplitWaves; ++i) {
+    m = max_nan(m, lm[i][r]);
+    mv = max(mv, lv[i]);
+  }
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSplitWaves; ++i) total += ll[i][r] * fast_exp2(lm[i][r] - m);
+  const float mine = fast_exp2(st.m - m) * __uint_as_float(kv_pow2_bits(st.mv - mv));
+  // rows that attended to nothing: sum 0, and zeros
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  float* rec = a.splits > 1 ? a.ws + (((int64_t)(w.b * (int64_t)a.c.Hkv + w.hk) * a.groups + group) * a.splits + split) * record_floats(D) : nullptr;
+  if (rec && wave == 0 && lane < 32) rec[(int64_t)kRows * D + r] = total == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(total);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = total == 0.f ? 0.f : ldexpf(st.o[c][4 * g + i] * (mine * inv), mv - 127 - kVBias);
+      *reinterpret_cast<f32x4*>(&lo[wave][r][8 * g + 4 * half]) = x;
+    }
+    __syncthreads();
+    // thread: row threadIdx / 8, four elements
+    const int rr = threadIdx.x >> 3, d = (threadIdx.x & 7) * 4;
+    f32x4 x = *reinterpret_cast<const f32x4*>(&lo[0][rr][d]);
+#pragma unroll
+    for (int i = 1; i < kSplitWaves; ++i) x += *reinterpret_cast<const f32x4*>(&lo[i][rr][d]);
+    if (rec) *reinterpret_cast<f32x4*>(rec + (int64_t)rr * D + 32 * c + d) = x;
+    else if (w.row0 + rr < w.rows) store_o4<T, D>(a, w, w.row0 + rr, 32 * c + d, x);
+  }
+}
+
+// The records of a row group's splits into its rows: thread: row, four elements.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a) {
+  constexpr int PER = 256 / (D / 4);  // rows of a workgroup
+  int id = blockIdx.x;
+  const int part = id % (kRows / PER);
+  id /= kRows / PER;
+  const int group = id % a.groups;
+  const int bh = id / a.groups;
+  Work w;
+  if (!kv_work(a, group, bh % a.c.Hkv, bh / a.c.Hkv, &w)) return;
+  const int r = part * PER + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  if (w.row0 + r >= w.rows) return;
+  const float* rec = a.ws + ((int64_t)bh * a.groups + group) * a.splits * record_floats(D);
+  float m = kMaxSeed;
+  for (int s = 0; s < a.splits; ++s) m = max_nan(m, rec[s * record_floats(D) + (int64_t)kRows * D + r]);
+  float total = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float z = fast_exp2(rec[s * record_floats(D) + (int64_t)kRows * D + r] - m);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(rec + s * record_floats(D) + (int64_t)r * D + d);
+    if (z != 0.f) x += y * z;
+    total += z;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  store_o4<T, D>(a, w, w.row0 + r, d, x * inv);
+}
+
+struct KvAttnPlan {
+  int groups, splits;
+  int64_t workgroups, ws_bytes;
+};
+
+KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
+  KvAttnPlan p;
+  const int G = a->H / a->cache.Hkv;
+  p.groups = (int)(((int64_t)a->seqs.max_rows * G + kRows - 1) / kRows);
+  const int64_t base = (int64_t)a->seqs.B * a->cache.Hkv * p.groups;
+  const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
+  const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
+  const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
+  int64_t splits = (2 * kCUs + base - 1) / base;
+  if (splits > (blocks + 7) / 8) splits = (blocks + 7) / 8;
+  if (splits < 1) splits = 1;
+  p.splits = (int)splits;
+  p.workgroups = base * splits;
+  p.ws_bytes = splits > 1 ? base * splits * record_floats(a->cache.D) * 4 : 0;
+  return p;
+}
+
+template <typename T, int D>
+hipError_t launch_kv_attn(const KvAttnParams& a, const KvAttnPlan& p, hipStream_t stream) {
+  hipLaunchKernelGGL((kv_attn_split_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kSplitWaves), 0, stream, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t merges = p.workgroups / p.splits * (kRows * (D / 4) / 256);
+  hipLaunchKernelGGL((kv_attn_merge_kernel<T, D>), dim3((unsigned)merges), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_kv_attn_t(const KvAttnParams& a, const KvAttnPlan& p, hipStream_t stream) {
+  return a.c.D == 64 ? launch_kv_attn<T, 64>(a, p, stream) : a.c.D == 128 ? launch_kv_attn<T, 128>(a, p, stream) : launch_kv_attn<T, 256>(a, p, stream);
+}
+
+// Checks; SA_OK with p->s.B == 0 for a call with nothing to do.
+int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan) {
+  if (a == nullptr) return fail(SA_ERR_INVALID, "args is NULL");
+  if (a->struct_size != sizeof(sa_kv_attn_args))
+    return fail(SA_ERR_INVALID, "struct_size %u does not match sizeof(sa_kv_attn_args) = %zu", a->struct_size, sizeof(sa_kv_attn_args));
+  int rc = kv_check_dtype(a->dtype);
+  if (rc == SA_OK) rc = kv_check_cache(a->cache);
+  if (rc == SA_OK) rc = kv_check_seqs(a->seqs);
+  if (rc != SA_OK) return rc;
+  if (a->H <= 0 || a->H % a->cache.Hkv) return fail(SA_ERR_INVALID, "H = %d must be a positive multiple of Hkv = %d", a->H, a->cache.Hkv);
+  if (a->H > (1 << 16)) return fail(SA_ERR_UNSUPPORTED, "%d heads (at most 65536)", a->H);
+  if (a->causal != 0 && a->causal != 1) return fail(SA_ERR_INVALID, "causal must be 0 or 1 (got %d)", a->causal);
+  if (!isfinite(a->scale)) return fail(SA_ERR_INVALID, "scale must be finite");
+  if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
+  *p = KvAttnParams{};
+  *plan = KvAttnPlan{0, 1, 0, 0};
+  if (kv_nothing(a->seqs)) return SA_OK;
+  const int size = kv_type_bytes(a->dtype);
+  const int64_t width = (int64_t)a->H * a->cache.D;
+  KvRows q, o;
+  rc = kv_rows(a->q, a->q_off, a->ldq, width, a->seqs.T, size, "q", &q);
+  if (rc == SA_OK) rc = kv_rows(a->o, a->o_off, a->ldo, width, a->seqs.T, size, "o", &o);
+  if (rc != SA_OK) return rc;
+  if (kv_overlap(q, o)) return fail(SA_ERR_ALIAS, "o overlaps q");
+  if (kv_overlap_cache(o, a->cache)) return fail(SA_ERR_ALIAS, "o overlaps the cache");
+  if (kv_overlap_seqs(o, a->seqs)) return fail(SA_ERR_ALIAS, "o overlaps the sequences' arrays");
+  const int G = a->H / a->cache.Hkv;
+  if ((int64_t)a->seqs.max_rows * G > (1 << 30)) return fail(SA_ERR_UNSUPPORTED, "%d rows of %d heads in one sequence", a->seqs.max_rows, G);
+  *plan = kv_attn_plan(a);
+  if (plan->workgroups > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%lld workgroups in one call", (long long)plan->workgroups);
+  p->c = a->cache;
+  p->s = a->seqs;
+  p->q = q.lo;
+  p->o = const_cast<char*>(o.lo);
+  p->ldq = q.ld;
+  p->ldo = o.ld;
+  p->scale_log2 = a->scale * kLog2e;
+  p->H = a->H;
+  p->G = G;
+  p->causal = a->causal;
+  p->groups = plan->groups;
+  p->splits = plan->splits;
+  p->aligned_q = (((uintptr_t)q.lo | (uintptr_t)q.ld) & 15) == 0;
+  p->aligned_o = (((uintptr_t)o.lo | (uintptr_t)o.ld) & 15) == 0;
+  return SA_OK;
+}
+
+}  // namespace
+
+}  // namespace sa
+
+using sa::fail;
+using sa::ok;
+
+extern "C" {
+
+int sa_kv_attention(const sa_kv_attn_args* args, void* stream) {
+  sa::KvAttnParams p;
+  sa::KvAttnPlan plan;
+  const int rc = sa::resolve_kv_attn(args, &p, &plan);
+  if (rc != SA_OK) return rc;
+  if (plan.workgroups == 0) return ok();
+  if (plan.ws_bytes > 0) {
+    if (!args->workspace || args->workspace_bytes < plan.ws_bytes)
+      return fail(SA_ERR_INVALID, "this call needs a device workspace of %lld bytes (sa_kv_attention_workspace_bytes)", (long long)plan.ws_bytes);
+    if ((uintptr_t)args->workspace & 15) return fail(SA_ERR_INVALID, "workspace must be 16-byte aligned");
+    const sa::KvRows q = {p.q, p.ldq, (int64_t)p.H * p.c.D * sa::kv_type_bytes(args->dtype), p.s.T};
+    const sa::KvRows o = {p.o, p.ldo, q.width, p.s.T}, ws = {(const char*)args->workspace, plan.ws_bytes, plan.ws_bytes, 1};
+    if (sa::kv_overlap(q, ws.lo, plan.ws_bytes) || sa::kv_overlap(o, ws.lo, plan.ws_bytes) || sa::kv_overlap_cache(ws, p.c) || sa::kv_overlap_seqs(ws, p.s))
+      return fail(SA_ERR_ALIAS, "the workspace overlaps q, o, the cache or the sequences' arrays");
+    p.ws = (float*)args->workspace;
+  }
+  const hipError_t e = args->dtype == SA_DT_F32   ? sa::launch_kv_attn_t<float>(p, plan, (hipStream_t)stream)
+                       : args->dtype == SA_DT_F16 ? sa::launch_kv_attn_t<_Float16>(p, plan, (hipStream_t)stream)
+                                                  : sa::launch_kv_attn_t<__bf16>(p, plan, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : sa::hip_fail(e, "kv_attention");
+}
+
+int64_t sa_kv_attention_workspace_bytes(const sa_kv_attn_args* args) {
+  sa::KvAttnParams p;
+  sa::KvAttnPlan plan;
+  const int rc = sa::resolve_kv_attn(args, &p, &plan);
+  if (rc != SA_OK) return rc;
+  ok();
+  return plan.ws_bytes;
+}
+
+int sa_kv_attention_shape(const sa_kv_attn_args* args, int32_t* rows, int32_t* splits) {
+  if (!rows || !splits) return fail(SA_ERR_INVALID, "rows and splits must be non-NULL");
+  sa::KvAttnParams p;
+  sa::KvAttnPlan plan;
+  const int rc = sa::resolve_kv_attn(args, &p, &plan);
+  if (rc != SA_OK) return rc;
+  *rows = sa::kRows;
+  *splits = plan.splits;
+  return ok();
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""ctypes binding of libsupra_attn.so (include/supra_attn.h, supra_linear.h, supra_vae.h).
+"""ctypes binding of libsupra_attn.so (include/supra_attn.h, supra_linear.h, supra_vae.h, supra_kv.h, supra_weights.h).
 
 Loading fails loudly when the library has not been built: there is no other implementation of the
 operator behind this module.
@@ -39,6 +39,13 @@ SA_EPI_STORE = 0
 SA_EPI_RESID = 1
 SA_EPI_RESID_GATE = 2
 
+# norms, rotation and the 8-bit cache (include/supra_kv.h)
+SA_NORM_NONE = 0
+SA_NORM_RMS = 1
+SA_ROPE_HALF = 0
+SA_ROPE_NEAR = 1
+SA_KV_BLOCK = 32
+
 # safetensors dtypes (include/supra_weights.h)
 SA_DT = {"OTHER": 0, "F32": 1, "F16": 2, "BF16": 3, "F64": 4, "I64": 5, "I32": 6, "I16": 7, "I8": 8, "U8": 9,
          "BOOL": 10, "U16": 11, "U32": 12, "U64": 13, "F8_E4M3": 14, "F8_E5M2": 15}
@@ -58,6 +65,13 @@ SIGNATURES = {
     "sa_linear_tile": (c_int, [c_void_p, POINTER(c_int32), POINTER(c_int32), POINTER(c_int32)]),
     "sa_vae_attention_f32": (c_int, [c_void_p, c_void_p]),
     "sa_vae_attention_workspace_bytes": (c_int64, [c_void_p]),
+    "sa_qk_norm_rope": (c_int, [c_void_p, c_void_p]),
+    "sa_kv_cache_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+    "sa_kv_write": (c_int, [c_void_p, c_void_p]),
+    "sa_kv_read": (c_int, [c_void_p, c_void_p]),
+    "sa_kv_attention": (c_int, [c_void_p, c_void_p]),
+    "sa_kv_attention_workspace_bytes": (c_int64, [c_void_p]),
+    "sa_kv_attention_shape": (c_int, [c_void_p, POINTER(c_int32), POINTER(c_int32)]),
     "sa_t5_bucket_lut": (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, POINTER(c_int32)]),
     "sa_t5_position_bias": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "sa_device_count": (c_int, [POINTER(c_int32)]),
@@ -263,6 +277,127 @@ class VaeAttnArgs(ctypes.Structure):
             setattr(self, name, val)
 
 
+class QkRopeArgs(ctypes.Structure):
+    """Mirror of sa_qk_rope_args (include/supra_kv.h)."""
+
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("T", c_int32),
+        ("H", c_int32),
+        ("Hkv", c_int32),
+        ("D", c_int32),
+        ("rotary_dim", c_int32),
+        ("pairs", c_int32),
+        ("norm", c_int32),
+        ("eps", c_float),
+        ("rope_scale", c_float),
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("q_off", c_int64),
+        ("k_off", c_int64),
+        ("ldq", c_int64),
+        ("ldk", c_int64),
+        ("q_out", c_void_p),
+        ("k_out", c_void_p),
+        ("qo_off", c_int64),
+        ("ko_off", c_int64),
+        ("ldqo", c_int64),
+        ("ldko", c_int64),
+        ("q_weight", c_void_p),
+        ("k_weight", c_void_p),
+        ("inv_freq", c_void_p),
+        ("positions", c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(QkRopeArgs)
+        for name, val in kw.items():
+            setattr(self, name, val)
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of sa_kv_cache (include/supra_kv.h)."""
+
+    _fields_ = [
+        ("pages", c_int32),
+        ("Hkv", c_int32),
+        ("D", c_int32),
+        ("reserved", c_int32),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+    ]
+
+
+class KvSeqs(ctypes.Structure):
+    """Mirror of sa_kv_seqs (include/supra_kv.h)."""
+
+    _fields_ = [
+        ("B", c_int32),
+        ("T", c_int32),
+        ("max_rows", c_int32),
+        ("max_blocks", c_int32),
+        ("row_start", c_void_p),
+        ("seq_len", c_void_p),
+        ("block_table", c_void_p),
+    ]
+
+
+class KvRowsArgs(ctypes.Structure):
+    """Mirror of sa_kv_rows_args (include/supra_kv.h)."""
+
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("cache", KvCache),
+        ("seqs", KvSeqs),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_off", c_int64),
+        ("v_off", c_int64),
+        ("ldk", c_int64),
+        ("ldv", c_int64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(KvRowsArgs)
+        for name, val in kw.items():
+            setattr(self, name, val)
+
+
+class KvAttnArgs(ctypes.Structure):
+    """Mirror of sa_kv_attn_args (include/supra_kv.h)."""
+
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("cache", KvCache),
+        ("seqs", KvSeqs),
+        ("H", c_int32),
+        ("causal", c_int32),
+        ("scale", c_float),
+        ("max_len", c_int32),
+        ("q", c_void_p),
+        ("o", c_void_p),
+        ("q_off", c_int64),
+        ("o_off", c_int64),
+        ("ldq", c_int64),
+        ("ldo", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(KvAttnArgs)
+        for name, val in kw.items():
+            setattr(self, name, val)
+
+
 class StTensor(ctypes.Structure):
     """sa_st_tensor: one safetensors header entry."""
 
@@ -367,6 +502,47 @@ def vae_workspace_bytes(args: VaeAttnArgs) -> int:
     if n < 0:
         raise SaError(int(n), lib.sa_last_error().decode())
     return int(n)
+
+
+def qk_norm_rope(args: QkRopeArgs, stream: int | None = None) -> None:
+    check(load().sa_qk_norm_rope(ctypes.byref(args), stream))
+
+
+def kv_cache_bytes(pages: int, Hkv: int, D: int) -> int:
+    """Bytes of a cache's k, and of its v."""
+    lib = load()
+    n = lib.sa_kv_cache_bytes(pages, Hkv, D)
+    if n < 0:
+        raise SaError(int(n), lib.sa_last_error().decode())
+    return int(n)
+
+
+def kv_write(args: KvRowsArgs, stream: int | None = None) -> None:
+    check(load().sa_kv_write(ctypes.byref(args), stream))
+
+
+def kv_read(args: KvRowsArgs, stream: int | None = None) -> None:
+    check(load().sa_kv_read(ctypes.byref(args), stream))
+
+
+def kv_attention(args: KvAttnArgs, stream: int | None = None) -> None:
+    check(load().sa_kv_attention(ctypes.byref(args), stream))
+
+
+def kv_attention_workspace_bytes(args: KvAttnArgs) -> int:
+    """Device scratch bytes sa_kv_attention needs for `args` (0 where no keys are split)."""
+    lib = load()
+    n = lib.sa_kv_attention_workspace_bytes(ctypes.byref(args))
+    if n < 0:
+        raise SaError(int(n), lib.sa_last_error().decode())
+    return int(n)
+
+
+def kv_attention_shape(args: KvAttnArgs) -> tuple[int, int]:
+    """(rows of a workgroup, workgroups that share their keys) of a call (sa_kv_attention_shape)."""
+    t = [c_int32(0) for _ in range(2)]
+    check(load().sa_kv_attention_shape(ctypes.byref(args), *(ctypes.byref(x) for x in t)))
+    return tuple(x.value for x in t)
 
 
 def workspace_bytes(args: AttnArgs) -> int:
