@@ -137,10 +137,10 @@ __device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int
   }
   auto sw = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   m = max(sw[0], sw[1]);
-  // factor 2^(14 - exponent of the largest): an infinity or NaN among them gives NaN scores, as in float32
+  // factor 2^(14 - exponent of the largest), with the scale's sign: an infinity or NaN among them gives NaN scores, as in float32
   const int f = min(127 + 14 + 127 - (int)(m >> 23), 253);
   q.exponent = 127 - f;
-  const float factor = __uint_as_float((uint32_t)f << 23);
+  const float factor = copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
@@ -162,30 +162,38 @@ struct State {
 // Bytes 0x7f and 0xff are NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// One page of 32 keys. kr, vr: its K and V tiles, 16 bytes of each KiB per lane. MASKED: of the page's keys each row
+// One page of 32 keys. k(c), v(c): the lane's 16 bytes of KiB c of its K and V tiles. MASKED: of the page's keys each row
 // attends to the first `limit` (its own).
-template <typename T, int D, bool MASKED>
-__device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const u32x4 (&kr)[D / 32], const u32x4 (&vr)[D / 32], int ke,
-                                     int ve, float scale_log2, int lane, int limit) {
+template <typename T, int D, bool MASKED, typename LoadK, typename LoadV>
+__device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const LoadK& k, const LoadV& v, int ke, int ve,
+                                     float scale_log2, int lane, int limit) {
   constexpr int NT = kTerms<T>;
   f32x16 s = zero16();
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    const f16x8 k0 = half8(kr[c][0], kr[c][1], 1.f), k1 = half8(kr[c][2], kr[c][3], 1.f);
+    const u32x4 x = k(c);
+    const f16x8 k0 = half8(x[0], x[1], 1.f), k1 = half8(x[2], x[3], 1.f);
 #pragma unroll
     for (int t = NT - 1; t >= 0; --t) {
       s = mfma(k0, q.t[c][0][t], s);
       s = mfma(k1, q.t[c][1][t], s);
     }
   }
-  const float f = ldexpf(scale_log2, q.exponent + ke - 127);
+  const float f = ldexpf(scale_log2, q.exponent + ke - 127);  // >= 0
   const int half = lane >> 5;
-  float top = -INFINITY;
+  float top;
+  if constexpr (MASKED) {
+    top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    s[i] *= f;
-    if constexpr (MASKED) s[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? s[i] : -INFINITY;
-    top = max_nan(top, s[i]);
+    for (int i = 0; i < 16; ++i) {
+      s[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? s[i] * f : -INFINITY;
+      top = max_nan(top, s[i]);
+    }
+  } else {
+    top = max_nan(s[0], s[1]);
+#pragma unroll
+    for (int i = 2; i < 16; ++i) top = max_nan(top, s[i]);
+    top *= f;
   }
   top = max_with_partner(top);
   const bool grows = !(top <= st.m + kLazy), v_grows = ve > st.mv;
@@ -203,38 +211,53 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const u
 #pragma unroll
       for (int i = 0; i < 16; ++i) st.o[c][i] *= r;
   }
-  float p[16];
+  const float base = (float)kPBias - st.m;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    p[i] = fast_exp2(s[i] - st.m + (float)kPBias);
-    st.l += p[i];
-  }
+  for (int i = 0; i < 16; ++i) s[i] = fast_exp2(MASKED ? s[i] + base : fmaf(s[i], f, base));
   f16x8 p0[NT], p1[NT];
-  split8<NT>(p, p0);
-  split8<NT>(p + 8, p1);
+  {
+    float p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = s[i];
+    split8<NT>(p, p0);
+    split8<NT>(p + 8, p1);
+    if constexpr (NT == 1) {
+      // the sum of the probabilities as they enter the product: two of them in one instruction, exact products
+      const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        st.l = __builtin_amdgcn_fdot2(f16x2{p0[0][i], p0[0][i + 1]}, one, st.l, false);
+        st.l = __builtin_amdgcn_fdot2(f16x2{p1[0][i], p1[0][i + 1]}, one, st.l, false);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.l += p[i];
+    }
+  }
   const float vs = __uint_as_float((uint32_t)max(ve - st.mv + kVBias + 127, 1) << 23);
-  u32x4 v[D / 32];
   bool nan_v = false;
   if constexpr (MASKED) {
     // A key that a row does not attend to may hold NaN in V, and 0 * NaN is not 0.
     uint32_t any = 0;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
+    for (int c = 0; c < D / 32; ++c) {
+      const u32x4 x = v(c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) any |= nan_bytes(vr[c][i]);
+      for (int i = 0; i < 4; ++i) any |= nan_bytes(x[i]);
+    }
     nan_v = __any(any != 0);
   }
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    v[c] = vr[c];
+    u32x4 x = v(c);
     if (MASKED && nan_v) {
       // NaN codes leave the tile, and a product of their places with the attended keys says whose sums they turn
       // into NaN.
       u32x4 at;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t n = nan_bytes(v[c][i]) >> 7, whole = n * 0xffu;
-        v[c][i] &= ~whole;
+        const uint32_t n = nan_bytes(x[i]) >> 7, whole = n * 0xffu;
+        x[i] &= ~whole;
         at[i] = n * 0x38u;  // the code of 1
       }
       float seen[16];
@@ -246,7 +269,7 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const u
 #pragma unroll
       for (int i = 0; i < 16; ++i) st.o[c][i] = hits[i] > 0.f ? NAN : st.o[c][i];
     }
-    const f16x8 v0 = half8(v[c][0], v[c][1], vs), v1 = half8(v[c][2], v[c][3], vs);
+    const f16x8 v0 = half8(x[0], x[1], vs), v1 = half8(x[2], x[3], vs);
 #pragma unroll
     for (int t = NT - 1; t >= 0; --t) {
       st.o[c] = mfma(v0, p0[t], st.o[c]);
@@ -313,8 +336,10 @@ __global__ __launch_bounds__(64 * kSplitWaves, D * kTerms<T> <= 128 ? 2 : 1) voi
 #pragma unroll
     for (int c = 0; c < C; ++c) vr[c] = *reinterpret_cast<const u32x4*>(a.c.v + at + c * 1024);
     const int ke = a.c.k_scale[(int64_t)page * a.c.Hkv + w.hk], ve = a.c.v_scale[(int64_t)page * a.c.Hkv + w.hk];
-    if ((blk + 1) * kKvBlock <= least) step<T, D, false>(q, st, kr, vr, ke, ve, a.scale_log2, lane, 0);
-    else step<T, D, true>(q, st, kr, vr, ke, ve, a.scale_log2, lane, limit - blk * kKvBlock);
+    const auto k = [&](int c) { return kr[c]; };
+    const auto v = [&](int c) { return vr[c]; };
+    if ((blk + 1) * kKvBlock <= least) step<T, D, false>(q, st, k, v, ke, ve, fabsf(a.scale_log2), lane, 0);
+    else step<T, D, true>(q, st, k, v, ke, ve, fabsf(a.scale_log2), lane, limit - blk * kKvBlock);
   }
 
   // ---- merge of the waves
@@ -362,36 +387,177 @@ __global__ __launch_bounds__(64 * kSplitWaves, D * kTerms<T> <= 128 ? 2 : 1) voi
   }
 }
 
-// The records of a row group's splits into its rows: thread: row, four elements.
+// ---- many rows: 128 of them to a workgroup, 32 to a wave, and the pages of all through LDS. A stage is kStage pages,
+// loaded to registers while the one before is worked on and then left in one of two LDS buffers, so a stage costs
+// one barrier; in LDS a lane's 16 bytes of a KiB lie at 16 * lane, which neither its write nor its read conflicts on.
+constexpr int kRowWaves = 4;
+constexpr int kStage = 2;
+
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a) {
-  constexpr int PER = 256 / (D / 4);  // rows of a workgroup
+__global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
+  constexpr int C = D / 32, ITEMS = kStage * 2 * C, MINE = ITEMS / kRowWaves;  // KiB of a stage, and a wave's
+  static_assert(ITEMS % kRowWaves == 0, "whole KiB per wave");
+  __shared__ __attribute__((aligned(16))) u32x4 tiles[2][ITEMS][64];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int id = blockIdx.x;
-  const int part = id % (kRows / PER);
-  id /= kRows / PER;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int wide = (a.groups + kRowWaves - 1) / kRowWaves;  // workgroups of a sequence's rows
+  const int block4 = id % wide;
+  id /= wide;
+  Work all, w;
+  if (!kv_work(a, block4 * kRowWaves, id % a.c.Hkv, id / a.c.Hkv, &all)) return;
+  w = all;
+  // pages of the workgroup: those of its last rows
+  {
+    const int last = min(block4 * kRowWaves + kRowWaves, (all.rows + kRows - 1) / kRows) - 1;
+    kv_work(a, last, all.hk, all.b, &all);
+  }
+  const bool on = kv_work(a, block4 * kRowWaves + wave, w.hk, w.b, &w);  // waves past the last rows only load
+  const int lo_block = (int)((int64_t)all.blocks * split / a.splits), hi_block = (int)((int64_t)all.blocks * (split + 1) / a.splits);
+
+  QTile<T, D> q;
+  State<D> st;
+  if (on) load_q<T, D>(a, w, lane, q);
+#pragma unroll
+  for (int c = 0; c < C; ++c) st.o[c] = zero16();
+  st.m = kMaxSeed;
+  st.l = 0.f;
+  st.mv = 0;
+  const int row = w.row0 + (lane & 31);
+  int limit = w.q.len, least = w.q.len;
+  if (a.causal) {
+    limit = min(limit, w.q.first + row / a.G + 1);
+    least = min(least, w.q.first + w.row0 / a.G + 1);
+  }
+
+  const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
+  const int place = (lane & 31) * 32 + (lane >> 5) * 16;
+  u32x4 part[MINE];
+  int pages[kStage], ke[kStage], ve[kStage];  // of the stage being loaded; a page that holds nothing: -1
+  const auto fetch = [&](int blk) {
+#pragma unroll
+    for (int p = 0; p < kStage; ++p) {
+      int page = -1;
+      if (blk + p < hi_block) page = table[blk + p];
+      pages[p] = kv_page_ok(page, a.c.pages) ? page : -1;
+      const int64_t at = (int64_t)max(pages[p], 0) * a.c.Hkv + w.hk;
+      ke[p] = a.c.k_scale[at];
+      ve[p] = a.c.v_scale[at];
+    }
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int item = wave + kRowWaves * j, p = item / (2 * C), c = item % C;
+      const bool is_v = item / C & 1;
+      int page = pages[0];
+#pragma unroll
+      for (int i = 1; i < kStage; ++i) page = p == i ? pages[i] : page;
+      const uint8_t* base = (is_v ? a.c.v : a.c.k) + kv_tile(max(page, 0), a.c.Hkv, w.hk, D);
+      part[j] = *reinterpret_cast<const u32x4*>(base + c * 1024 + place);
+    }
+  };
+  const auto leave = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) tiles[buf][wave + kRowWaves * j][lane] = part[j];
+  };
+
+  if (lo_block < hi_block) {
+    fetch(lo_block);
+    leave(0);
+  }
+  int buf = 0;
+  for (int blk = lo_block; blk < hi_block; blk += kStage, buf ^= 1) {
+    int now[kStage], kn[kStage], vn[kStage];
+#pragma unroll
+    for (int p = 0; p < kStage; ++p) now[p] = pages[p], kn[p] = ke[p], vn[p] = ve[p];
+    __syncthreads();
+    const bool more = blk + kStage < hi_block;
+    if (more) fetch(blk + kStage);
+    if (on) {
+#pragma unroll
+      for (int p = 0; p < kStage; ++p) {
+        if (now[p] < 0 || blk + p >= w.blocks) continue;
+        const auto k = [&](int c) { return tiles[buf][p * 2 * C + c][lane]; };
+        const auto v = [&](int c) { return tiles[buf][p * 2 * C + C + c][lane]; };
+        const int kk = __builtin_amdgcn_readfirstlane(kn[p]), vv = __builtin_amdgcn_readfirstlane(vn[p]);
+        if ((blk + p + 1) * kKvBlock <= least) step<T, D, false>(q, st, k, v, kk, vv, fabsf(a.scale_log2), lane, 0);
+        else step<T, D, true>(q, st, k, v, kk, vv, fabsf(a.scale_log2), lane, limit - (blk + p) * kKvBlock);
+      }
+    }
+    if (more) leave(buf ^ 1);
+  }
+  if (!on) return;
+
+  const float total = sum_with_partner(st.l);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int half = lane >> 5;
+  float* rec = a.splits > 1 ? a.ws + (((int64_t)(w.b * (int64_t)a.c.Hkv + w.hk) * a.groups + w.row0 / kRows) * a.splits + split) * record_floats(D) : nullptr;
+  if (rec && half == 0) rec[(int64_t)kRows * D + lane] = total == 0.f ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = total == 0.f ? 0.f : ldexpf(st.o[c][4 * g + i] * inv, st.mv - 127 - kVBias);
+      const int d = 32 * c + 8 * g + 4 * half;
+      if (rec) *reinterpret_cast<f32x4*>(rec + (int64_t)(lane & 31) * D + d) = x;
+      else if (row < w.rows) store_o4<T, D>(a, w, row, d, x);
+    }
+  }
+}
+
+// The records of a row's splits into the row, a workgroup for each row: the weights of its splits in LDS, then D/4
+// threads to a record and 1024 / D records at a time, joined through LDS.
+constexpr int kMaxSplits = 512;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int rows) {
+  constexpr int W = D / 4, SIDE = 256 / W;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float wave_m[4], wave_l[4];
+  __shared__ __attribute__((aligned(16))) f32x4 parts[SIDE][W];
+  int id = blockIdx.x;
+  const int r = id % rows;
+  id /= rows;
   const int group = id % a.groups;
   const int bh = id / a.groups;
   Work w;
   if (!kv_work(a, group, bh % a.c.Hkv, bh / a.c.Hkv, &w)) return;
-  const int r = part * PER + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   if (w.row0 + r >= w.rows) return;
   const float* rec = a.ws + ((int64_t)bh * a.groups + group) * a.splits * record_floats(D);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const float* sums = rec + (int64_t)kRows * D + r;
   float m = kMaxSeed;
-  for (int s = 0; s < a.splits; ++s) m = max_nan(m, rec[s * record_floats(D) + (int64_t)kRows * D + r]);
-  float total = 0.f;
+  for (int s = tid; s < a.splits; s += 256) m = max_nan(m, weight[s] = sums[s * record_floats(D)]);
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) m = max_nan(m, __shfl_xor(m, i));
+  if (lane == 0) wave_m[tid >> 6] = m;
+  __syncthreads();
+  m = max_nan(max_nan(wave_m[0], wave_m[1]), max_nan(wave_m[2], wave_m[3]));
+  float l = 0.f;
+  for (int s = tid; s < a.splits; s += 256) l += weight[s] = fast_exp2(weight[s] - m);
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i);
+  if (lane == 0) wave_l[tid >> 6] = l;
+  __syncthreads();
+  l = wave_l[0] + wave_l[1] + wave_l[2] + wave_l[3];
+  const int side = tid / W, d = tid % W * 4;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float z = fast_exp2(rec[s * record_floats(D) + (int64_t)kRows * D + r] - m);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(rec + s * record_floats(D) + (int64_t)r * D + d);
-    if (z != 0.f) x += y * z;
-    total += z;
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  store_o4<T, D>(a, w, w.row0 + r, d, x * inv);
+#pragma unroll 4
+  for (int s = side; s < a.splits; s += SIDE) x += *reinterpret_cast<const f32x4*>(rec + s * record_floats(D) + (int64_t)r * D + d) * weight[s];
+  parts[side][d / 4] = x;
+  __syncthreads();
+  if (side > 0) return;
+#pragma unroll
+  for (int i = 1; i < SIDE; ++i) x += parts[i][d / 4];
+  store_o4<T, D>(a, w, w.row0 + r, d, x * (l == 0.f ? 0.f : 1.f / l));
 }
 
 struct KvAttnPlan {
   int groups, splits;
+  bool many;  // the kernel of many rows
   int64_t workgroups, ws_bytes;
 };
 
@@ -399,7 +565,8 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   KvAttnPlan p;
   const int G = a->H / a->cache.Hkv;
   p.groups = (int)(((int64_t)a->seqs.max_rows * G + kRows - 1) / kRows);
-  const int64_t base = (int64_t)a->seqs.B * a->cache.Hkv * p.groups;
+  p.many = p.groups > 2;
+  const int64_t base = (int64_t)a->seqs.B * a->cache.Hkv * (p.many ? (p.groups + kRowWaves - 1) / kRowWaves : p.groups);
   const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
@@ -408,17 +575,20 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   if (splits < 1) splits = 1;
   p.splits = (int)splits;
   p.workgroups = base * splits;
-  p.ws_bytes = splits > 1 ? base * splits * record_floats(a->cache.D) * 4 : 0;
+  p.ws_bytes = splits > 1 ? (int64_t)a->seqs.B * a->cache.Hkv * p.groups * splits * record_floats(a->cache.D) * 4 : 0;
   return p;
 }
 
 template <typename T, int D>
 hipError_t launch_kv_attn(const KvAttnParams& a, const KvAttnPlan& p, hipStream_t stream) {
-  hipLaunchKernelGGL((kv_attn_split_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kSplitWaves), 0, stream, a);
+  if (p.many) hipLaunchKernelGGL((kv_attn_rows_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kRowWaves), 0, stream, a);
+  else hipLaunchKernelGGL((kv_attn_split_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kSplitWaves), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  const int64_t merges = p.workgroups / p.splits * (kRows * (D / 4) / 256);
-  hipLaunchKernelGGL((kv_attn_merge_kernel<T, D>), dim3((unsigned)merges), dim3(256), 0, stream, a);
+  const int64_t most = (int64_t)a.s.max_rows * a.G;
+  const int rows = (int)(most < kRows ? most : kRows);
+  const int64_t merges = (int64_t)a.s.B * a.c.Hkv * p.groups * rows;  // below 2^31: splits > 1 bounds the groups
+  hipLaunchKernelGGL((kv_attn_merge_kernel<T, D>), dim3((unsigned)merges), dim3(256), 0, stream, a, rows);
   return hipGetLastError();
 }
 
@@ -442,7 +612,7 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   if (!isfinite(a->scale)) return fail(SA_ERR_INVALID, "scale must be finite");
   if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
   *p = KvAttnParams{};
-  *plan = KvAttnPlan{0, 1, 0, 0};
+  *plan = KvAttnPlan{0, 1, false, 0, 0};
   if (kv_nothing(a->seqs)) return SA_OK;
   const int size = kv_type_bytes(a->dtype);
   const int64_t width = (int64_t)a->H * a->cache.D;
@@ -520,7 +690,7 @@ int sa_kv_attention_shape(const sa_kv_attn_args* args, int32_t* rows, int32_t* s
   sa::KvAttnPlan plan;
   const int rc = sa::resolve_kv_attn(args, &p, &plan);
   if (rc != SA_OK) return rc;
-  *rows = sa::kRows;
+  *rows = plan.many ? sa::kRows * sa::kRowWaves : sa::kRows;
   *splits = plan.splits;
   return ok();
 }

@@ -4,12 +4,16 @@
 // lanes, so a wave works on several heads at once and the sum of squares is a few exchanges inside the group. A
 // lane's chunk is P pairs of the rotation: P elements and their P partners (or 2P neighbours), both in its own
 // registers, so the rotation exchanges nothing; the elements past rotary_dim are cut into pairs the same way and
-// turned by no angle. A lane keeps the same pairs for every head, so it forms their sines and cosines once.
+// turned by no angle. A lane keeps the same pairs for every head, so a token's sines and cosines are formed once, one
+// pair to a lane, and handed out through LDS (every lane forming its own: 48.5 us against 39.1 at 8191 tokens x 40 heads
+// x 128 in bfloat16, 14.8 against 7.5 at 777 x 9 x 256). The next step's rows are loaded before this one's are worked on.
 //
 // Angles: position * inv_freq in float64, in turns, less the nearest whole turn (exact); what is left is at most half a
 // turn and goes on in float32, so position 2^20 is as good as position 1. sincospif of twice that.
 //
-// Bound: HBM traffic, every element read and written once.
+// Bound: HBM traffic, every element read and written once: 168 MB in 39.6 us, 4.2 TB/s (8191 x 40 x 128, bfloat16);
+// 151 MB in 33.3 us, 4.5 TB/s (16384 x 18 x 64, float32), where a copy of 4 GiB reaches 4.6. Down to some hundred
+// tokens, latency: 6.6 us at 777 x 9 x 256, 4.2 us of kernel at one token.
 
 #include <hip/hip_runtime.h>
 
@@ -24,6 +28,9 @@ namespace sa {
 namespace {
 
 constexpr int kRopeWaves = 4;
+constexpr int kRopeMaxPairs = 256;  // D is at most 512
+constexpr int kRopePairs = 4;       // pairs of a lane: 16 bytes of float32, 8 of a 16-bit type (8 pairs, 16 bytes of one, take
+                                    // twice the registers: 16384 x 18 heads x 64 in bfloat16 23.5 us against 20.7)
 
 struct RopeParams {
   const char* q;  // rows, offsets included; strides in bytes
@@ -86,60 +93,86 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_kernel(RopeParams a) 
 
   const int in_group = lane & (a.group - 1), sub = lane >> a.shift, step = 64 >> a.shift;
   int pa[N], pb[N];
-  bool has[N];
-  float cs[N][P], sn[N][P], wq[N][2 * P], wk[N][2 * P];
-  const double at = a.half > 0 ? (double)a.positions[t] : 0.0;
+  bool has[N], turned[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int p = (n * a.group + in_group) * P;  // the chunk's first pair
     has[n] = 2 * p < a.D;
-    const bool turned = p < a.half;
-    const int rest = a.D / 2 - a.half;  // pairs past the rotated ones
+    turned[n] = p < a.half;
     if constexpr (NEAR) {
       pa[n] = 2 * p;
       pb[n] = 2 * p + 1;
     } else {
-      pa[n] = turned ? p : p + a.half;
-      pb[n] = pa[n] + (turned ? a.half : rest);
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      float c = 1.f, s = 0.f;
-      if (has[n] && turned) {
-        double f = at * a.inv_freq[p + i] * 0.15915494309189533576888;  // turns: 1 / (2 pi)
-        f -= rint(f);
-        sincospif(2.f * (float)f, &s, &c);
-        c *= a.rope_scale;
-        s *= a.rope_scale;
-      }
-      cs[n][i] = c;
-      sn[n][i] = s;
-      const int d0 = pa[n] + (NEAR ? 2 * i : i), d1 = pb[n] + (NEAR ? 2 * i : i);
-      wq[n][i] = has[n] && a.wq ? a.wq[d0] : 1.f;
-      wq[n][P + i] = has[n] && a.wq ? a.wq[d1] : 1.f;
-      wk[n][i] = has[n] && a.wk ? a.wk[d0] : 1.f;
-      wk[n][P + i] = has[n] && a.wk ? a.wk[d1] : 1.f;
+      pa[n] = turned[n] ? p : p + a.half;
+      pb[n] = pa[n] + (turned[n] ? a.half : a.D / 2 - a.half);
     }
   }
 
-  for (int h0 = first; h0 < last; h0 += step) {
+  // The rows of one step: a head for each group of lanes. Groups past the last head run along (the exchanges need
+  // all lanes) with zeros.
+  const auto load = [&](int h0, float (&u)[N][P], float (&v)[N][P]) {
     const int h = h0 + sub;
-    const bool on = h < last;  // groups past the last head run along: the exchanges need all lanes
     const bool is_k = h >= a.H;
-    const int hh = is_k ? h - a.H : h;
-    const T* x = reinterpret_cast<const T*>((is_k ? a.k : a.q) + t * (is_k ? a.ldk : a.ldq)) + (int64_t)hh * a.D;
-    T* y = reinterpret_cast<T*>((is_k ? a.ko : a.qo) + t * (is_k ? a.ldko : a.ldqo)) + (int64_t)hh * a.D;
-    float u[N][P], v[N][P], ss = 0.f;
+    const T* x = reinterpret_cast<const T*>((is_k ? a.k : a.q) + t * (is_k ? a.ldk : a.ldq)) + (int64_t)(is_k ? h - a.H : h) * a.D;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int i = 0; i < P; ++i) u[n][i] = v[n][i] = 0.f;
-      if (on && has[n]) load_pairs<T, P, NEAR, ALIGNED>(x, pa[n], pb[n], u[n], v[n]);
-#pragma unroll
-      for (int i = 0; i < P; ++i) ss = fmaf(u[n][i], u[n][i], fmaf(v[n][i], v[n][i], ss));
+      if (h < last && has[n]) load_pairs<T, P, NEAR, ALIGNED>(x, pa[n], pb[n], u[n], v[n]);
     }
+  };
+  float u[N][P], v[N][P];
+  load(first, u, v);
+
+  // Weights of the lane's places, and the token's sines and cosines: lane i forms those of pairs i, i + 64, ... once
+  // for the wave, and each lane takes its own from LDS (the wave's own part of it: its accesses are in order).
+  float wq[N][2][P], wk[N][2][P], cs[N][P], sn[N][P];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) wq[n][0][i] = wq[n][1][i] = wk[n][0][i] = wk[n][1][i] = 1.f;
+    if (has[n] && a.wq) load_pairs<float, P, NEAR, ALIGNED>(a.wq, pa[n], pb[n], wq[n][0], wq[n][1]);
+    if (has[n] && a.wk) load_pairs<float, P, NEAR, ALIGNED>(a.wk, pa[n], pb[n], wk[n][0], wk[n][1]);
+  }
+  __shared__ __attribute__((aligned(16))) float turns[kRopeWaves][2][kRopeMaxPairs];
+  float(&mine)[2][kRopeMaxPairs] = turns[threadIdx.x >> 6];
+  if (a.half > 0) {
+    const double at = (double)a.positions[t];
+    for (int p = lane; p < a.half; p += 64) {
+      double f = at * a.inv_freq[p] * 0.15915494309189533576888;  // turns: 1 / (2 pi)
+      f -= rint(f);
+      float s, c;
+      sincospif(2.f * (float)f, &s, &c);
+      mine[0][p] = c * a.rope_scale;
+      mine[1][p] = s * a.rope_scale;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int p = (n * a.group + in_group) * P;
+#pragma unroll
+    for (int i = 0; i < P; ++i) cs[n][i] = 1.f, sn[n][i] = 0.f;
+    if (turned[n]) {
+      load_row<float, P, ALIGNED>(&mine[0][p], cs[n]);
+      load_row<float, P, ALIGNED>(&mine[1][p], sn[n]);
+    }
+  }
+
+  for (int h0 = first; h0 < last; h0 += step) {
+    float nu[N][P], nv[N][P];
+    load(h0 + step, nu, nv);  // past the last head: zeros
+    const int h = h0 + sub;
+    const bool is_k = h >= a.H;
+    T* y = reinterpret_cast<T*>((is_k ? a.ko : a.qo) + t * (is_k ? a.ldko : a.ldqo)) + (int64_t)(is_k ? h - a.H : h) * a.D;
     float r = 1.f;
     if (a.norm == SA_NORM_RMS) {
+      float ss = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < P; ++i) ss = fmaf(u[n][i], u[n][i], fmaf(v[n][i], v[n][i], ss));
       for (int m = 1; m < a.group; m <<= 1) ss += __shfl_xor(ss, m);
       r = 1.f / sqrtf(ss * a.inv_d + a.eps);
     }
@@ -147,28 +180,25 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_kernel(RopeParams a) 
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const float p = u[n][i] * r * (is_k ? wk[n][i] : wq[n][i]), q = v[n][i] * r * (is_k ? wk[n][P + i] : wq[n][P + i]);
+        const float p = u[n][i] * r * (is_k ? wk[n][0][i] : wq[n][0][i]), q = v[n][i] * r * (is_k ? wk[n][1][i] : wq[n][1][i]);
         u[n][i] = p * cs[n][i] - q * sn[n][i];
         v[n][i] = q * cs[n][i] + p * sn[n][i];
       }
-      if (on && has[n]) store_pairs<T, P, NEAR, ALIGNED>(y, pa[n], pb[n], u[n], v[n]);
+      if (h < last && has[n]) store_pairs<T, P, NEAR, ALIGNED>(y, pa[n], pb[n], u[n], v[n]);
+#pragma unroll
+      for (int i = 0; i < P; ++i) u[n][i] = nu[n][i], v[n][i] = nv[n][i];
     }
   }
 }
 
 template <typename T, bool NEAR>
-hipError_t launch_rope(const RopeParams& a, int P, unsigned grid, hipStream_t stream) {
-  if (P > 1) {
-    constexpr int kP = 16 / (int)sizeof(T) > 4 ? 8 : 4;
-    if (P == kP) hipLaunchKernelGGL((qk_rope_kernel<T, kP, 1, NEAR>), dim3(grid), dim3(64 * kRopeWaves), 0, stream, a);
-    else return hipErrorInvalidValue;
-  } else {
-    hipLaunchKernelGGL((qk_rope_kernel<T, 1, 4, NEAR>), dim3(grid), dim3(64 * kRopeWaves), 0, stream, a);
-  }
+hipError_t launch_rope(const RopeParams& a, bool vec, unsigned grid, hipStream_t stream) {
+  if (vec) hipLaunchKernelGGL((qk_rope_kernel<T, kRopePairs, 1, NEAR>), dim3(grid), dim3(64 * kRopeWaves), 0, stream, a);
+  else hipLaunchKernelGGL((qk_rope_kernel<T, 1, 4, NEAR>), dim3(grid), dim3(64 * kRopeWaves), 0, stream, a);
   return hipGetLastError();
 }
 
-int resolve_rope(const sa_qk_rope_args* a, RopeParams* p, int* pairs_per_lane) {
+int resolve_rope(const sa_qk_rope_args* a, RopeParams* p, bool* vector) {
   if (a == nullptr) return fail(SA_ERR_INVALID, "args is NULL");
   if (a->struct_size != sizeof(sa_qk_rope_args))
     return fail(SA_ERR_INVALID, "struct_size %u does not match sizeof(sa_qk_rope_args) = %zu", a->struct_size, sizeof(sa_qk_rope_args));
@@ -234,19 +264,18 @@ int resolve_rope(const sa_qk_rope_args* a, RopeParams* p, int* pairs_per_lane) {
   p->inv_d = 1.f / (float)a->D;
   p->rope_scale = a->rope_scale == 0.f ? 1.f : a->rope_scale;
 
-  // Vector accesses where every chunk of P pairs stays on one side of the rotated part and every access is aligned;
+  // Vector accesses where every chunk of pairs stays on one side of the rotated part and every access is aligned;
   // single elements otherwise (any even D, any alignment).
-  const int P = size == 2 ? 8 : 4;
   const uintptr_t bits = (uintptr_t)q.lo | (uintptr_t)k.lo | (uintptr_t)qo.lo | (uintptr_t)ko.lo | (uintptr_t)q.ld | (uintptr_t)k.ld |
-                         (uintptr_t)qo.ld | (uintptr_t)ko.ld;
-  const bool vec = bits % 16 == 0 && p->half % P == 0 && (a->D / 2) % P == 0 && (a->D * size) % 16 == 0;
-  *pairs_per_lane = vec ? P : 1;
-  const int chunks = a->D / 2 / *pairs_per_lane, most = vec ? 1 : 4;  // chunks of a lane
+                         (uintptr_t)qo.ld | (uintptr_t)ko.ld | (uintptr_t)a->q_weight | (uintptr_t)a->k_weight;
+  const bool vec = bits % 16 == 0 && p->half % kRopePairs == 0 && a->D % (2 * kRopePairs) == 0;
+  const int chunks = a->D / 2 / (vec ? kRopePairs : 1), most = vec ? 1 : 4;  // of a head, and of a lane
   p->group = 1;
   while (p->group * most < chunks || (!vec && p->group < 64 && p->group < chunks)) {
     p->group *= 2;
     p->shift++;
   }
+  *vector = vec;
   return SA_OK;
 }
 
@@ -259,14 +288,16 @@ using sa::ok;
 
 extern "C" int sa_qk_norm_rope(const sa_qk_rope_args* args, void* stream) {
   sa::RopeParams p;
-  int P = 1;
-  const int rc = sa::resolve_rope(args, &p, &P);
+  bool vec = false;
+  const int rc = sa::resolve_rope(args, &p, &vec);
   if (rc != SA_OK) return rc;
   if (p.T == 0 || p.heads == 0) return ok();
-  // A wave takes all heads of a token (its angles are formed once) unless the tokens alone leave the device short
-  // of waves: then a token's heads are cut into runs, down to one step of the wave.
+  // A wave takes all heads of a token (its angles and weights are fetched once) unless the tokens alone leave the
+  // device short of waves: then a token's heads are cut into runs, down to one step of the wave. Enough is one
+  // wave per SIMD and then some for 16-bit rows (8191 tokens x 40 heads x 128, whole tokens / runs of one step:
+  // 39.6 / 42.5 us), many more for float32 rows, whose steps move twice the bytes (73.5 / 63.6 us).
   const int step = 64 / p.group, steps = (p.heads + step - 1) / step;
-  const int64_t want = 4096;  // waves: four for each SIMD
+  const int64_t want = args->dtype == SA_DT_F32 ? 40000 : 4096;
   int64_t runs = p.T >= want ? 1 : (want + p.T - 1) / p.T;
   if (runs > steps) runs = steps;
   const int per = (int)((steps + runs - 1) / runs);
@@ -278,8 +309,8 @@ extern "C" int sa_qk_norm_rope(const sa_qk_rope_args* args, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
   const unsigned grid = (unsigned)groups;
   hipError_t e;
-  if (args->dtype == SA_DT_F32) e = near ? sa::launch_rope<float, true>(p, P, grid, s) : sa::launch_rope<float, false>(p, P, grid, s);
-  else if (args->dtype == SA_DT_F16) e = near ? sa::launch_rope<_Float16, true>(p, P, grid, s) : sa::launch_rope<_Float16, false>(p, P, grid, s);
-  else e = near ? sa::launch_rope<__bf16, true>(p, P, grid, s) : sa::launch_rope<__bf16, false>(p, P, grid, s);
+  if (args->dtype == SA_DT_F32) e = near ? sa::launch_rope<float, true>(p, vec, grid, s) : sa::launch_rope<float, false>(p, vec, grid, s);
+  else if (args->dtype == SA_DT_F16) e = near ? sa::launch_rope<_Float16, true>(p, vec, grid, s) : sa::launch_rope<_Float16, false>(p, vec, grid, s);
+  else e = near ? sa::launch_rope<__bf16, true>(p, vec, grid, s) : sa::launch_rope<__bf16, false>(p, vec, grid, s);
   return e == hipSuccess ? ok() : sa::hip_fail(e, "qk_norm_rope");
 }
