@@ -89,24 +89,32 @@ __device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32
 // What a workgroup works on.
 struct Work {
   KvSeq q;
-  int b, hk, row0, rows;  // packed rows [row0, row0 + 32) of rows * G
+  int b, hk, row0, rows;  // packed rows from row0 on, of `rows` in all (tokens * G)
   int blocks;             // pages that any of its rows attends to
 };
 
-__device__ __forceinline__ bool kv_work(const KvAttnParams& a, int group, int hk, int b, Work* w) {
+__device__ __forceinline__ bool kv_work(const KvAttnParams& a, int rows, int group, int hk, int b, Work* w) {
   w->q = kv_seq(a.s, b);
   w->b = b;
   w->hk = hk;
-  w->row0 = group * kRows;
+  w->row0 = group * rows;
   w->rows = w->q.rows * a.G;
   if (w->row0 >= w->rows) return false;
   int keys = w->q.len;
   if (a.causal) {
-    const int t = (min(w->row0 + kRows, w->rows) - 1) / a.G;  // the last row's token
+    const int t = (min(w->row0 + rows, w->rows) - 1) / a.G;  // the last row's token
     keys = max(0, min(keys, w->q.first + t + 1));
   }
   w->blocks = (keys + kKvBlock - 1) / kKvBlock;
   return true;
+}
+
+// Factor that brings a row whose largest magnitude has the bits m to float16: 2^(14 - its exponent), with the scale's
+// sign; the row is 2^exponent times that. An infinity or NaN in it gives NaN scores, as in float32.
+__device__ __forceinline__ float q_factor(const KvAttnParams& a, uint32_t m, int& exponent) {
+  const int f = min(127 + 14 + 127 - (int)(m >> 23), 253);
+  exponent = 127 - f;
+  return copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
 }
 
 // Q's operand for one 32-row group: lane (row = lane & 31, half): elements 32c + 16 half .. + 16 of each chunk c.
@@ -137,10 +145,7 @@ __device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int
   }
   auto sw = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   m = max(sw[0], sw[1]);
-  // factor 2^(14 - exponent of the largest), with the scale's sign: an infinity or NaN among them gives NaN scores, as in float32
-  const int f = min(127 + 14 + 127 - (int)(m >> 23), 253);
-  q.exponent = 127 - f;
-  const float factor = copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
+  const float factor = q_factor(a, m, q.exponent);
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
@@ -159,8 +164,13 @@ struct State {
   int mv;  // exponent byte of V's reference scale
 };
 
-// Bytes 0x7f and 0xff are NaN.
+// Codes 0x7f and 0xff are NaN: bit 7 of their bytes.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+  const uint32_t n = nan_bytes(w);
+  return w & ~(n | (n - (n >> 7)));
+}
+__device__ __forceinline__ uint32_t ones_at_nan(uint32_t w) { return (nan_bytes(w) >> 7) * 0x38u; }  // 0x38: the code of 1
 
 // One page of 32 keys. k(c), v(c): the lane's 16 bytes of KiB c of its K and V tiles. MASKED: of the page's keys each row
 // attends to the first `limit` (its own).
@@ -169,9 +179,20 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const L
                                      float scale_log2, int lane, int limit) {
   constexpr int NT = kTerms<T>;
   f32x16 s = zero16();
+  // Where registers allow, the whole page is on its way before the first product (the compiler would fetch V's part
+  // after the exponentials: 630 us against 619 for 4 x 2048 rows over 4096 keys at 32 heads x 128).
+  constexpr bool EARLY = D <= 128;
+  u32x4 kr[D / 32], vr[D / 32];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) kr[c] = k(c);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) vr[c] = v(c);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    const u32x4 x = k(c);
+    const u32x4 x = EARLY ? kr[c] : k(c);
     const f16x8 k0 = half8(x[0], x[1], 1.f), k1 = half8(x[2], x[3], 1.f);
 #pragma unroll
     for (int t = NT - 1; t >= 0; --t) {
@@ -249,25 +270,10 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const L
   }
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    u32x4 x = v(c);
+    u32x4 x = EARLY ? vr[c] : v(c);
     if (MASKED && nan_v) {
-      // NaN codes leave the tile, and a product of their places with the attended keys says whose sums they turn
-      // into NaN.
-      u32x4 at;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t n = nan_bytes(x[i]) >> 7, whole = n * 0xffu;
-        x[i] &= ~whole;
-        at[i] = n * 0x38u;  // the code of 1
-      }
-      float seen[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) seen[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? 1.f : 0.f;
-      f32x16 hits = zero16();
-      hits = mfma(half8(at[0], at[1], 1.f), round8(seen), hits);
-      hits = mfma(half8(at[2], at[3], 1.f), round8(seen + 8), hits);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.o[c][i] = hits[i] > 0.f ? NAN : st.o[c][i];
+      for (int i = 0; i < 4; ++i) x[i] = without_nan(x[i]);
     }
     const f16x8 v0 = half8(x[0], x[1], vs), v1 = half8(x[2], x[3], vs);
 #pragma unroll
@@ -276,10 +282,29 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const L
       st.o[c] = mfma(v1, p1[t], st.o[c]);
     }
   }
+  if (MASKED && nan_v) {
+    // The places of the NaN codes, which left the tile, times the attended keys: whose sums they turn into NaN.
+    float seen[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) seen[i] = 8 * (i >> 2) + 4 * half + (i & 3) < limit ? 1.f : 0.f;
+    const f16x8 s0 = round8(seen), s1 = round8(seen + 8);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      u32x4 x = v(c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = ones_at_nan(x[i]);
+      const f32x16 hits = mfma(half8(x[2], x[3], 1.f), s1, mfma(half8(x[0], x[1], 1.f), s0, zero16()));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[c][i] = hits[i] > 0.f ? NAN : st.o[c][i];
+    }
+  }
 }
 
-// A split's record: 32 rows of D floats, then their 32 log2-sums.
-constexpr int64_t record_floats(int D) { return (int64_t)kRows * (D + 1); }
+// A split's record of a group of `rows` rows: rows x D floats, then their log2-sums.
+__host__ __device__ constexpr int64_t record_floats(int rows, int D) { return (int64_t)rows * (D + 1); }
+__device__ __forceinline__ int64_t record_at(const KvAttnParams& a, int b, int hk, int group, int split, int rows, int D) {
+  return ((((int64_t)b * a.c.Hkv + hk) * a.groups + group) * a.splits + split) * record_floats(rows, D);
+}
 
 template <typename T, int D>
 __device__ __forceinline__ void store_o4(const KvAttnParams& a, const Work& w, int row, int d, f32x4 x) {
@@ -289,13 +314,194 @@ __device__ __forceinline__ void store_o4(const KvAttnParams& a, const Work& w, i
   else store_row<T, 4, false>(p, y);
 }
 
+// ---- few rows: 16 or 32 of them to a workgroup, whose waves take the pages in turn and are merged at the end. Tiles of
+// 16x16x32 instructions: S^T of 16 keys x 16 rows leaves the keys 4 kq + i of a tile in lane (row, kq = lane >> 4), and the
+// two tiles of a page take its tokens in the order that makes those of one lane eight neighbouring codes of V:
+// tile u, place p: token 16 ((p >> 2) & 1) + 8 u + 4 (p >> 3) + (p & 3).
 constexpr int kSplitWaves = 4;
 
+__device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ int token16(int u, int p) { return 16 * (p >> 2 & 1) + 8 * u + 4 * (p >> 3) + (p & 3); }
+
+// One page's codes as a lane needs them: K: of pair i of 32-channel chunks and tile u, 16 channels of one token
+// (channels 64 i + 16 kq on); V: of channel 16 e + (lane & 15), eight tokens.
+template <int D>
+struct Page16 {
+  u32x4 k[D / 64][2];
+  uint2 v[D / 16];
+  int ke, ve;
+  bool ok;
+};
+
+template <int D>
+__device__ __forceinline__ void load_page(const KvAttnParams& a, int hk, int32_t id, int lane, Page16<D>& p) {
+  p.ok = kv_page_ok(id, a.c.pages);
+  const int64_t head = (int64_t)(p.ok ? id : 0) * a.c.Hkv + hk, at = head * (kKvBlock * D);
+  const int kq = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      p.k[i][u] = *reinterpret_cast<const u32x4*>(a.c.k + at + (2 * i + (kq >> 1)) * 1024 + token16(u, lane & 15) * 32 + (kq & 1) * 16);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) p.v[e] = *reinterpret_cast<const uint2*>(a.c.v + at + (16 * e + (lane & 15)) * 32 + 8 * kq);
+  p.ke = a.c.k_scale[head];
+  p.ve = a.c.v_scale[head];
+}
+
+// 16 rows: Q's operand, O^T (channel 16 e + 4 kq + i of row lane & 15), maximum and this lane's sum.
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kSplitWaves, D * kTerms<T> <= 128 ? 2 : 1) void kv_attn_split_kernel(KvAttnParams a) {
-  constexpr int C = D / 32, PAD = 36;
-  __shared__ __attribute__((aligned(16))) float lo[kSplitWaves][kRows][PAD];
-  __shared__ float lm[kSplitWaves][kRows], ll[kSplitWaves][kRows];
+struct Rows16 {
+  f16x8 q[D / 64][2][kTerms<T>];  // channels 64 i + 16 kq + 8 m on
+  f32x4 o[D / 16];
+  float m, l;
+  int exponent, limit;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void load_rows16(const KvAttnParams& a, const Work& w, int row, int lane, Rows16<T, D>& st) {
+  const int r = row + (lane & 15), kq = lane >> 4;
+  const bool on = r < w.rows;
+  const T* p = nullptr;
+  if (on) p = reinterpret_cast<const T*>(a.q + (int64_t)(w.q.row0 + r / a.G) * a.ldq) + (int64_t)(w.hk * a.G + r % a.G) * D + 16 * kq;
+  float x[D / 64][16];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[i][j] = 0.f;
+    if (on) {
+      if (a.aligned_q) load_row<T, 16, true>(p + 64 * i, x[i]);
+      else load_row<T, 16, false>(p + 64 * i, x[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7fffffffu);
+  }
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+  const float factor = q_factor(a, m, st.exponent);
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[i][j] *= factor;
+    split8<kTerms<T>>(x[i], st.q[i][0]);
+    split8<kTerms<T>>(x[i] + 8, st.q[i][1]);
+  }
+  st.limit = w.q.len;
+  if (a.causal) st.limit = min(st.limit, w.q.first + r / a.G + 1);
+  st.m = kMaxSeed;
+  st.l = 0.f;
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) st.o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// One page (number blk) for N groups of 16 rows; mv as in State.
+template <typename T, int D, int N, bool MASKED>
+__device__ __forceinline__ void step16(const Page16<D>& pg, Rows16<T, D> (&st)[N], int& mv, float scale_log2, int lane, int blk) {
+  constexpr int NT = kTerms<T>;
+  const int kq = lane >> 4, ke = __builtin_amdgcn_readfirstlane(pg.ke), ve = __builtin_amdgcn_readfirstlane(pg.ve);
+  f32x4 s[N][2];
+#pragma unroll
+  for (int n = 0; n < N; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const u32x4 x = pg.k[i][u];
+      const f16x8 k0 = half8(x[0], x[1], 1.f), k1 = half8(x[2], x[3], 1.f);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int t = NT - 1; t >= 0; --t) {
+          s[n][u] = mfma16(k0, st[n].q[i][0][t], s[n][u]);
+          s[n][u] = mfma16(k1, st[n].q[i][1][t], s[n][u]);
+        }
+    }
+  const bool v_grows = ve > mv;
+  const float v_factor = v_grows ? __uint_as_float(kv_pow2_bits(mv - ve)) : 1.f;
+  if (v_grows) mv = ve;
+  f16x8 p[N][NT];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float f = ldexpf(scale_log2, st[n].exponent + ke - 127);
+    float z[8], top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[n][u][i] * f;
+        if constexpr (MASKED) x = blk * kKvBlock + token16(u, 4 * kq + i) < st[n].limit ? x : -INFINITY;
+        z[4 * u + i] = x;
+        top = max_nan(top, x);
+      }
+    top = max_over_rows4(top);
+    const bool grows = !(top <= st[n].m + kLazy);
+    if (__any(grows) || v_grows) {
+      const float m = grows ? max_nan(st[n].m, top) : st[n].m;
+      const float r = fast_exp2(st[n].m - m);
+      st[n].l *= r;
+      st[n].m = m;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) st[n].o[e] *= r * v_factor;
+    }
+    const float base = (float)kPBias - st[n].m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      z[i] = fast_exp2(z[i] + base);
+      if constexpr (NT == 2) st[n].l += z[i];
+    }
+    split8<NT>(z, p[n]);
+    if constexpr (NT == 1) {
+      const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) st[n].l = __builtin_amdgcn_fdot2(f16x2{p[n][0][i], p[n][0][i + 1]}, one, st[n].l, false);
+    }
+  }
+  const float vs = __uint_as_float((uint32_t)max(ve - mv + kVBias + 127, 1) << 23);
+  bool nan_v = false;
+  if constexpr (MASKED) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) any |= nan_bytes(pg.v[e].x) | nan_bytes(pg.v[e].y);
+    nan_v = __any(any != 0);
+  }
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) {
+    uint32_t x = pg.v[e].x, y = pg.v[e].y;
+    if (MASKED && nan_v) {
+      x = without_nan(x);
+      y = without_nan(y);
+    }
+    const f16x8 v = half8(x, y, vs);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int t = NT - 1; t >= 0; --t) st[n].o[e] = mfma16(v, p[n][t], st[n].o[e]);
+  }
+  if (MASKED && nan_v) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float seen[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) seen[i] = blk * kKvBlock + token16(i >> 2, 4 * kq + (i & 3)) < st[n].limit ? 1.f : 0.f;
+      const f16x8 sn = round8(seen);
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        const f32x4 hits = mfma16(half8(ones_at_nan(pg.v[e].x), ones_at_nan(pg.v[e].y), 1.f), sn, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[n].o[e][i] = hits[i] > 0.f ? NAN : st[n].o[e][i];
+      }
+    }
+  }
+}
+
+template <typename T, int D, int N>
+__global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_split_kernel(KvAttnParams a) {
+  constexpr int ROWS = 16 * N, PAD = 20;
+  __shared__ __attribute__((aligned(16))) float lo[2][kSplitWaves][ROWS][PAD];
+  __shared__ float lm[kSplitWaves][ROWS], ll[kSplitWaves][ROWS];
   __shared__ int lv[kSplitWaves];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -305,85 +511,97 @@ __global__ __launch_bounds__(64 * kSplitWaves, D * kTerms<T> <= 128 ? 2 : 1) voi
   const int group = id % a.groups;
   id /= a.groups;
   Work w;
-  if (!kv_work(a, group, id % a.c.Hkv, id / a.c.Hkv, &w)) return;
+  if (!kv_work(a, ROWS, group, id % a.c.Hkv, id / a.c.Hkv, &w)) return;
   const int lo_block = (int)((int64_t)w.blocks * split / a.splits), hi_block = (int)((int64_t)w.blocks * (split + 1) / a.splits);
 
-  QTile<T, D> q;
-  load_q<T, D>(a, w, lane, q);
-  State<D> st;
-#pragma unroll
-  for (int c = 0; c < C; ++c) st.o[c] = zero16();
-  st.m = kMaxSeed;
-  st.l = 0.f;
-  st.mv = 0;
-
-  // The row's own limit: keys [0, limit) of the sequence.
-  const int row = w.row0 + (lane & 31);
-  int limit = w.q.len;
-  if (a.causal) limit = min(limit, w.q.first + row / a.G + 1);
-  int least = w.q.len;  // the least of the group's rows
-  if (a.causal) least = min(least, w.q.first + w.row0 / a.G + 1);
-
   const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
-  const int place = (lane & 31) * 32 + (lane >> 5) * 16;
-  for (int blk = lo_block + wave; blk < hi_block; blk += kSplitWaves) {
-    const int32_t page = table[blk];
-    if (!kv_page_ok(page, a.c.pages)) continue;
-    const int64_t at = kv_tile(page, a.c.Hkv, w.hk, D) + place;
-    u32x4 kr[C], vr[C];
+  int blk = lo_block + wave;
+  Page16<D> pg[2];
+  int32_t next = -1;  // the id of the page after the one being loaded
+  if (blk < hi_block) {
+    const int32_t first = table[blk];
+    if (blk + kSplitWaves < hi_block) next = table[blk + kSplitWaves];
+    load_page<D>(a, w.hk, first, lane, pg[0]);
+  }
+  Rows16<T, D> st[N];
 #pragma unroll
-    for (int c = 0; c < C; ++c) kr[c] = *reinterpret_cast<const u32x4*>(a.c.k + at + c * 1024);
-#pragma unroll
-    for (int c = 0; c < C; ++c) vr[c] = *reinterpret_cast<const u32x4*>(a.c.v + at + c * 1024);
-    const int ke = a.c.k_scale[(int64_t)page * a.c.Hkv + w.hk], ve = a.c.v_scale[(int64_t)page * a.c.Hkv + w.hk];
-    const auto k = [&](int c) { return kr[c]; };
-    const auto v = [&](int c) { return vr[c]; };
-    if ((blk + 1) * kKvBlock <= least) step<T, D, false>(q, st, k, v, ke, ve, fabsf(a.scale_log2), lane, 0);
-    else step<T, D, true>(q, st, k, v, ke, ve, fabsf(a.scale_log2), lane, limit - blk * kKvBlock);
+  for (int n = 0; n < N; ++n) load_rows16<T, D>(a, w, w.row0 + 16 * n, lane, st[n]);
+  int mv = 0;
+  const float scale = fabsf(a.scale_log2);
+  // Pages that every row attends to as a whole, two at a time, each loaded while the one before is worked on; what is
+  // left (a whole one perhaps, then the cut ones) follows with the masks.
+  int least = w.q.len;
+  if (a.causal) least = max(0, min(least, w.q.first + w.row0 / a.G + 1));
+  const int whole = min(hi_block, least / kKvBlock);
+  const auto load_next = [&](int at, Page16<D>& p) {
+    const int32_t now = next;
+    next = at + kSplitWaves < hi_block ? table[at + kSplitWaves] : -1;
+    load_page<D>(a, w.hk, now, lane, p);
+  };
+  while (blk + kSplitWaves < whole) {
+    load_next(blk + kSplitWaves, pg[1]);
+    if (pg[0].ok) step16<T, D, N, false>(pg[0], st, mv, scale, lane, blk);
+    blk += kSplitWaves;
+    load_next(blk + kSplitWaves, pg[0]);  // past the last page: page 0, not used
+    if (pg[1].ok) step16<T, D, N, false>(pg[1], st, mv, scale, lane, blk);
+    blk += kSplitWaves;
+  }
+  while (blk < hi_block) {
+    const bool more = blk + kSplitWaves < hi_block;
+    if (more) load_next(blk + kSplitWaves, pg[1]);
+    if (pg[0].ok) step16<T, D, N, true>(pg[0], st, mv, scale, lane, blk);
+    pg[0] = pg[1];
+    blk += kSplitWaves;
   }
 
   // ---- merge of the waves
-  const float l = sum_with_partner(st.l);
-  if (lane < 32) {
-    lm[wave][lane] = st.m;
-    ll[wave][lane] = l;
+  const int r = lane & 15, kq = lane >> 4;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float l = sum_over_rows4(st[n].l);
+    if (lane < 16) {
+      lm[wave][16 * n + lane] = st[n].m;
+      ll[wave][16 * n + lane] = l;
+    }
   }
-  if (lane == 0) lv[wave] = st.mv;
+  if (lane == 0) lv[wave] = mv;
   __syncthreads();
-  const int r = lane & 31, half = lane >> 5;
-  float m = lm[0][r];
-  int mv = lv[0];
+  float* rec = a.splits > 1 ? a.ws + record_at(a, w.b, w.hk, group, split, ROWS, D) : nullptr;
+  int top_v = lv[0];
 #pragma unroll
-  for (int i = 1; i < kSplitWaves; ++i) {
-    m = max_nan(m, lm[i][r]);
-    mv = max(mv, lv[i]);
+  for (int i = 1; i < kSplitWaves; ++i) top_v = max(top_v, lv[i]);
+  float mine[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float m = lm[0][16 * n + r], total = 0.f;
+#pragma unroll
+    for (int i = 1; i < kSplitWaves; ++i) m = max_nan(m, lm[i][16 * n + r]);
+#pragma unroll
+    for (int i = 0; i < kSplitWaves; ++i) total += ll[i][16 * n + r] * fast_exp2(lm[i][16 * n + r] - m);
+    // rows that attended to nothing: sum 0, and zeros
+    mine[n] = total == 0.f ? 0.f : fast_exp2(st[n].m - m) * __uint_as_float(kv_pow2_bits(mv - top_v)) / total;
+    if (rec && wave == 0 && lane < 16) rec[ROWS * D + 16 * n + lane] = total == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(total);
   }
-  float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < kSplitWaves; ++i) total += ll[i][r] * fast_exp2(lm[i][r] - m);
-  const float mine = fast_exp2(st.m - m) * __uint_as_float(kv_pow2_bits(st.mv - mv));
-  // rows that attended to nothing: sum 0, and zeros
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  float* rec = a.splits > 1 ? a.ws + (((int64_t)(w.b * (int64_t)a.c.Hkv + w.hk) * a.groups + group) * a.splits + split) * record_floats(D) : nullptr;
-  if (rec && wave == 0 && lane < 32) rec[(int64_t)kRows * D + r] = total == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(total);
+  for (int e = 0; e < D / 16; ++e) {
+    float(&half)[kSplitWaves][ROWS][PAD] = lo[e & 1];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    if (c > 0) __syncthreads();
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int n = 0; n < N; ++n) {
       f32x4 x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = total == 0.f ? 0.f : ldexpf(st.o[c][4 * g + i] * (mine * inv), mv - 127 - kVBias);
-      *reinterpret_cast<f32x4*>(&lo[wave][r][8 * g + 4 * half]) = x;
+      for (int i = 0; i < 4; ++i) x[i] = ldexpf(st[n].o[e][i] * mine[n], top_v - 127 - kVBias);
+      *reinterpret_cast<f32x4*>(&half[wave][16 * n + r][4 * kq]) = x;
     }
     __syncthreads();
-    // thread: row threadIdx / 8, four elements
-    const int rr = threadIdx.x >> 3, d = (threadIdx.x & 7) * 4;
-    f32x4 x = *reinterpret_cast<const f32x4*>(&lo[0][rr][d]);
+    // thread: row, four channels; the other buffer takes the next 16 channels meanwhile
+    const int rr = threadIdx.x >> 2, d = (threadIdx.x & 3) * 4;
+    if (rr < ROWS) {
+      f32x4 x = *reinterpret_cast<const f32x4*>(&half[0][rr][d]);
 #pragma unroll
-    for (int i = 1; i < kSplitWaves; ++i) x += *reinterpret_cast<const f32x4*>(&lo[i][rr][d]);
-    if (rec) *reinterpret_cast<f32x4*>(rec + (int64_t)rr * D + 32 * c + d) = x;
-    else if (w.row0 + rr < w.rows) store_o4<T, D>(a, w, w.row0 + rr, 32 * c + d, x);
+      for (int i = 1; i < kSplitWaves; ++i) x += *reinterpret_cast<const f32x4*>(&half[i][rr][d]);
+      if (rec) *reinterpret_cast<f32x4*>(rec + rr * D + 16 * e + d) = x;
+      else if (w.row0 + rr < w.rows) store_o4<T, D>(a, w, w.row0 + rr, 16 * e + d, x);
+    }
   }
 }
 
@@ -394,7 +612,7 @@ constexpr int kRowWaves = 4;
 constexpr int kStage = 2;
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
+__global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
   constexpr int C = D / 32, ITEMS = kStage * 2 * C, MINE = ITEMS / kRowWaves;  // KiB of a stage, and a wave's
   static_assert(ITEMS % kRowWaves == 0, "whole KiB per wave");
   __shared__ __attribute__((aligned(16))) u32x4 tiles[2][ITEMS][64];
@@ -404,17 +622,18 @@ __global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void 
   const int split = id % a.splits;
   id /= a.splits;
   const int wide = (a.groups + kRowWaves - 1) / kRowWaves;  // workgroups of a sequence's rows
-  const int block4 = id % wide;
-  id /= wide;
+  const int heads = a.s.B * a.c.Hkv;
+  const int block4 = wide - 1 - id / heads;
+  id %= heads;
   Work all, w;
-  if (!kv_work(a, block4 * kRowWaves, id % a.c.Hkv, id / a.c.Hkv, &all)) return;
+  if (!kv_work(a, kRows, block4 * kRowWaves, id % a.c.Hkv, id / a.c.Hkv, &all)) return;
   w = all;
   // pages of the workgroup: those of its last rows
   {
     const int last = min(block4 * kRowWaves + kRowWaves, (all.rows + kRows - 1) / kRows) - 1;
-    kv_work(a, last, all.hk, all.b, &all);
+    kv_work(a, kRows, last, all.hk, all.b, &all);
   }
-  const bool on = kv_work(a, block4 * kRowWaves + wave, w.hk, w.b, &w);  // waves past the last rows only load
+  const bool on = kv_work(a, kRows, block4 * kRowWaves + wave, w.hk, w.b, &w);  // waves past the last rows only load
   const int lo_block = (int)((int64_t)all.blocks * split / a.splits), hi_block = (int)((int64_t)all.blocks * (split + 1) / a.splits);
 
   QTile<T, D> q;
@@ -426,22 +645,22 @@ __global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void 
   st.l = 0.f;
   st.mv = 0;
   const int row = w.row0 + (lane & 31);
-  int limit = w.q.len, least = w.q.len;
-  if (a.causal) {
-    limit = min(limit, w.q.first + row / a.G + 1);
-    least = min(least, w.q.first + w.row0 / a.G + 1);
-  }
+  int limit = w.q.len;
+  if (a.causal) limit = min(limit, w.q.first + row / a.G + 1);
 
   const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
   const int place = (lane & 31) * 32 + (lane >> 5) * 16;
   u32x4 part[MINE];
   int pages[kStage], ke[kStage], ve[kStage];  // of the stage being loaded; a page that holds nothing: -1
+  int32_t ids[kStage];  // of the stage after that: a page's loads wait for its id, so it comes a stage earlier
+  const auto look = [&](int blk) {
+#pragma unroll
+    for (int p = 0; p < kStage; ++p) ids[p] = blk + p < hi_block ? table[blk + p] : -1;
+  };
   const auto fetch = [&](int blk) {
 #pragma unroll
     for (int p = 0; p < kStage; ++p) {
-      int page = -1;
-      if (blk + p < hi_block) page = table[blk + p];
-      pages[p] = kv_page_ok(page, a.c.pages) ? page : -1;
+      pages[p] = kv_page_ok(ids[p], a.c.pages) ? ids[p] : -1;
       const int64_t at = (int64_t)max(pages[p], 0) * a.c.Hkv + w.hk;
       ke[p] = a.c.k_scale[at];
       ve[p] = a.c.v_scale[at];
@@ -456,6 +675,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void 
       const uint8_t* base = (is_v ? a.c.v : a.c.k) + kv_tile(max(page, 0), a.c.Hkv, w.hk, D);
       part[j] = *reinterpret_cast<const u32x4*>(base + c * 1024 + place);
     }
+    look(blk + kStage);
   };
   const auto leave = [&](int buf) {
 #pragma unroll
@@ -463,36 +683,46 @@ __global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void 
   };
 
   if (lo_block < hi_block) {
+    look(lo_block);
     fetch(lo_block);
     leave(0);
   }
+  // Stages that every row of the workgroup attends to as a whole, then the others.
+  const float scale = fabsf(a.scale_log2);
   int buf = 0;
-  for (int blk = lo_block; blk < hi_block; blk += kStage, buf ^= 1) {
-    int now[kStage], kn[kStage], vn[kStage];
+  const auto stages = [&](int begin, int end, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    for (int blk = begin; blk < end; blk += kStage, buf ^= 1) {
+      int now[kStage], kn[kStage], vn[kStage];
 #pragma unroll
-    for (int p = 0; p < kStage; ++p) now[p] = pages[p], kn[p] = ke[p], vn[p] = ve[p];
-    __syncthreads();
-    const bool more = blk + kStage < hi_block;
-    if (more) fetch(blk + kStage);
-    if (on) {
+      for (int p = 0; p < kStage; ++p) now[p] = pages[p], kn[p] = ke[p], vn[p] = ve[p];
+      __syncthreads();
+      const bool more = blk + kStage < hi_block;
+      if (more) fetch(blk + kStage);
+      if (on) {
 #pragma unroll
-      for (int p = 0; p < kStage; ++p) {
-        if (now[p] < 0 || blk + p >= w.blocks) continue;
-        const auto k = [&](int c) { return tiles[buf][p * 2 * C + c][lane]; };
-        const auto v = [&](int c) { return tiles[buf][p * 2 * C + C + c][lane]; };
-        const int kk = __builtin_amdgcn_readfirstlane(kn[p]), vv = __builtin_amdgcn_readfirstlane(vn[p]);
-        if ((blk + p + 1) * kKvBlock <= least) step<T, D, false>(q, st, k, v, kk, vv, fabsf(a.scale_log2), lane, 0);
-        else step<T, D, true>(q, st, k, v, kk, vv, fabsf(a.scale_log2), lane, limit - (blk + p) * kKvBlock);
+        for (int p = 0; p < kStage; ++p) {
+          if (now[p] < 0 || (MASKED && blk + p >= w.blocks)) continue;
+          const auto k = [&](int c) { return tiles[buf][p * 2 * C + c][lane]; };
+          const auto v = [&](int c) { return tiles[buf][p * 2 * C + C + c][lane]; };
+          const int kk = __builtin_amdgcn_readfirstlane(kn[p]), vv = __builtin_amdgcn_readfirstlane(vn[p]);
+          step<T, D, MASKED>(q, st, k, v, kk, vv, scale, lane, limit - (blk + p) * kKvBlock);
+        }
       }
+      if (more) leave(buf ^ 1);
     }
-    if (more) leave(buf ^ 1);
-  }
+  };
+  int least = w.q.len;  // keys that the workgroup's first row attends to
+  if (a.causal) least = max(0, min(least, w.q.first + block4 * kRowWaves * kRows / a.G + 1));
+  const int whole = max(lo_block, lo_block + (min(hi_block, least / kKvBlock) - lo_block) / kStage * kStage);
+  stages(lo_block, whole, std::false_type{});
+  stages(whole, hi_block, std::true_type{});
   if (!on) return;
 
   const float total = sum_with_partner(st.l);
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int half = lane >> 5;
-  float* rec = a.splits > 1 ? a.ws + (((int64_t)(w.b * (int64_t)a.c.Hkv + w.hk) * a.groups + w.row0 / kRows) * a.splits + split) * record_floats(D) : nullptr;
+  float* rec = a.splits > 1 ? a.ws + record_at(a, w.b, w.hk, w.row0 / kRows, split, kRows, D) : nullptr;
   if (rec && half == 0) rec[(int64_t)kRows * D + lane] = total == 0.f ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -513,7 +743,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D * kTerms<T> <= 128 ? 2 : 1) void 
 constexpr int kMaxSplits = 512;
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int rows) {
+__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int group_rows, int rows) {
   constexpr int W = D / 4, SIDE = 256 / W;
   __shared__ float weight[kMaxSplits];
   __shared__ float wave_m[4], wave_l[4];
@@ -524,13 +754,14 @@ __global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int 
   const int group = id % a.groups;
   const int bh = id / a.groups;
   Work w;
-  if (!kv_work(a, group, bh % a.c.Hkv, bh / a.c.Hkv, &w)) return;
+  if (!kv_work(a, group_rows, group, bh % a.c.Hkv, bh / a.c.Hkv, &w)) return;
   if (w.row0 + r >= w.rows) return;
-  const float* rec = a.ws + ((int64_t)bh * a.groups + group) * a.splits * record_floats(D);
+  const float* rec = a.ws + record_at(a, bh / a.c.Hkv, bh % a.c.Hkv, group, 0, group_rows, D);
+  const int64_t next = record_floats(group_rows, D);
   const int tid = threadIdx.x, lane = tid & 63;
-  const float* sums = rec + (int64_t)kRows * D + r;
+  const float* sums = rec + (int64_t)group_rows * D + r;
   float m = kMaxSeed;
-  for (int s = tid; s < a.splits; s += 256) m = max_nan(m, weight[s] = sums[s * record_floats(D)]);
+  for (int s = tid; s < a.splits; s += 256) m = max_nan(m, weight[s] = sums[s * next]);
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) m = max_nan(m, __shfl_xor(m, i));
   if (lane == 0) wave_m[tid >> 6] = m;
@@ -546,7 +777,7 @@ __global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int 
   const int side = tid / W, d = tid % W * 4;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = side; s < a.splits; s += SIDE) x += *reinterpret_cast<const f32x4*>(rec + s * record_floats(D) + (int64_t)r * D + d) * weight[s];
+  for (int s = side; s < a.splits; s += SIDE) x += *reinterpret_cast<const f32x4*>(rec + s * next + (int64_t)r * D + d) * weight[s];
   parts[side][d / 4] = x;
   __syncthreads();
   if (side > 0) return;
@@ -556,16 +787,18 @@ __global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int 
 }
 
 struct KvAttnPlan {
-  int groups, splits;
-  bool many;  // the kernel of many rows
+  int group_rows, groups, splits;  // of a row group; row groups of a sequence and key head; workgroups that share their keys
+  bool many;                       // the kernel of many rows
   int64_t workgroups, ws_bytes;
 };
 
 KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   KvAttnPlan p;
   const int G = a->H / a->cache.Hkv;
-  p.groups = (int)(((int64_t)a->seqs.max_rows * G + kRows - 1) / kRows);
-  p.many = p.groups > 2;
+  const int64_t rows = (int64_t)a->seqs.max_rows * G;
+  p.many = rows > 64;
+  p.group_rows = p.many ? kRows : rows <= 16 || a->cache.D == 256 ? 16 : 32;
+  p.groups = (int)((rows + p.group_rows - 1) / p.group_rows);
   const int64_t base = (int64_t)a->seqs.B * a->cache.Hkv * (p.many ? (p.groups + kRowWaves - 1) / kRowWaves : p.groups);
   const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
@@ -575,20 +808,22 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   if (splits < 1) splits = 1;
   p.splits = (int)splits;
   p.workgroups = base * splits;
-  p.ws_bytes = splits > 1 ? (int64_t)a->seqs.B * a->cache.Hkv * p.groups * splits * record_floats(a->cache.D) * 4 : 0;
+  p.ws_bytes = splits > 1 ? (int64_t)a->seqs.B * a->cache.Hkv * p.groups * splits * record_floats(p.group_rows, a->cache.D) * 4 : 0;
   return p;
 }
 
 template <typename T, int D>
 hipError_t launch_kv_attn(const KvAttnParams& a, const KvAttnPlan& p, hipStream_t stream) {
-  if (p.many) hipLaunchKernelGGL((kv_attn_rows_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kRowWaves), 0, stream, a);
-  else hipLaunchKernelGGL((kv_attn_split_kernel<T, D>), dim3((unsigned)p.workgroups), dim3(64 * kSplitWaves), 0, stream, a);
+  const dim3 grid((unsigned)p.workgroups);
+  if (p.many) hipLaunchKernelGGL((kv_attn_rows_kernel<T, D>), grid, dim3(64 * kRowWaves), 0, stream, a);
+  else if (p.group_rows == 16) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 1>), grid, dim3(64 * kSplitWaves), 0, stream, a);
+  else if constexpr (D <= 128) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 2>), grid, dim3(64 * kSplitWaves), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t most = (int64_t)a.s.max_rows * a.G;
-  const int rows = (int)(most < kRows ? most : kRows);
+  const int rows = (int)(most < p.group_rows ? most : p.group_rows);
   const int64_t merges = (int64_t)a.s.B * a.c.Hkv * p.groups * rows;  // below 2^31: splits > 1 bounds the groups
-  hipLaunchKernelGGL((kv_attn_merge_kernel<T, D>), dim3((unsigned)merges), dim3(256), 0, stream, a, rows);
+  hipLaunchKernelGGL((kv_attn_merge_kernel<T, D>), dim3((unsigned)merges), dim3(256), 0, stream, a, p.group_rows, rows);
   return hipGetLastError();
 }
 
@@ -612,7 +847,7 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   if (!isfinite(a->scale)) return fail(SA_ERR_INVALID, "scale must be finite");
   if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
   *p = KvAttnParams{};
-  *plan = KvAttnPlan{0, 1, false, 0, 0};
+  *plan = KvAttnPlan{kRows, 0, 1, false, 0, 0};
   if (kv_nothing(a->seqs)) return SA_OK;
   const int size = kv_type_bytes(a->dtype);
   const int64_t width = (int64_t)a->H * a->cache.D;
@@ -690,7 +925,7 @@ int sa_kv_attention_shape(const sa_kv_attn_args* args, int32_t* rows, int32_t* s
   sa::KvAttnPlan plan;
   const int rc = sa::resolve_kv_attn(args, &p, &plan);
   if (rc != SA_OK) return rc;
-  *rows = plan.many ? sa::kRows * sa::kRowWaves : sa::kRows;
+  *rows = plan.many ? sa::kRows * sa::kRowWaves : plan.group_rows;
   *splits = plan.splits;
   return ok();
 }

@@ -264,16 +264,17 @@ def test_cache_bytes():
 
 def test_splits_follow_rows_and_keys():
     """Few rows over long caches are split, at eight pages at least to a share; many rows are not; and the workspace is
-    a record of 32 rows for each share."""
+    a record of each group of 16 or 32 rows for each share."""
     for H, Hkv, D, B, n, keys in ((32, 8, 128, 1, 1, 777), (32, 8, 128, 64, 1, 8191), (4, 4, 64, 2, 3, 131072), (8, 1, 256, 1, 2048, 4096), (2, 1, 64, 1, 1, 32)):
         s = seqs(B=B, T=B * n, max_rows=n, max_blocks=-(-keys // 32))
         a = attn_args(cache(Hkv=Hkv, D=D, pages=1 << 10, v=FAKE + (1 << 36), k_scale=FAKE + (2 << 36), v_scale=FAKE + (3 << 36)), s, H=H,
                       q=FAKE + (4 << 36), o=FAKE + (5 << 36))
         rows, splits = _lib.kv_attention_shape(a)
-        assert rows % 32 == 0
-        groups = -(-n * (H // Hkv) // 32)
+        assert rows in (16, 32, 128)
+        record = min(rows, 32)
+        groups = -(-n * (H // Hkv) // record)
         assert splits == 1 or splits * 8 <= -(-keys // 32) + 7
-        assert _lib.kv_attention_workspace_bytes(a) == (0 if splits == 1 else B * Hkv * groups * splits * 32 * (D + 1) * 4)
+        assert _lib.kv_attention_workspace_bytes(a) == (0 if splits == 1 else B * Hkv * groups * splits * record * (D + 1) * 4)
 
 
 def test_oracle_codes_are_torch_codes():
