@@ -32,7 +32,7 @@ struct KvMove {
   char* v;
   int64_t ldk, ldv;  // bytes
   int blocks;        // tiles of one head that a sequence's rows can touch
-  int64_t tiles;     // B * blocks * Hkv * 2
+  uint32_t tiles;    // B * blocks * Hkv * 2
 };
 
 // The tile of one wave: (sequence, block of 32 positions, head, K or V). Consecutive waves take the heads of one
@@ -46,13 +46,14 @@ struct Tile {
   int32_t page;   // -1: none
 };
 
-__device__ __forceinline__ bool kv_tile_of(const KvMove& a, int64_t i, Tile* t) {
+__device__ __forceinline__ bool kv_tile_of(const KvMove& a, uint32_t i, Tile* t) {
   if (i >= a.tiles) return false;
   t->is_v = i & 1;
   i >>= 1;
-  t->h = (int)(i % a.c.Hkv);
-  i /= a.c.Hkv;
-  const int n = (int)(i % a.blocks), b = (int)(i / a.blocks);
+  const uint32_t heads = (uint32_t)a.c.Hkv, blocks = (uint32_t)a.blocks;
+  t->h = (int)(i % heads);
+  i /= heads;
+  const int n = (int)(i % blocks), b = (int)(i / blocks);
   t->q = kv_seq(a.s, b);
   const KvSeq& q = t->q;
   if (q.rows == 0) return false;
@@ -72,67 +73,176 @@ __device__ __forceinline__ bool kv_tile_of(const KvMove& a, int64_t i, Tile* t) 
   return true;
 }
 
-// Bits of |x| for the scale: infinities and NaN do not count.
-__device__ __forceinline__ uint32_t amax_bits(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
-}
-
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t y = __shfl_xor(x, m);
-    x = x > y ? x : y;
-  }
+  for (int m = 1; m < 64; m <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, m));
   return x;
 }
 
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+// Two neighbouring elements as they come from memory, and what the kernels do to them: the larger magnitude, two
+// codes at a scale, two elements of two codes.
+template <typename T>
+struct Pair {
+  uint32_t w;
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint16_t kInf = __is_same(T, __bf16) ? 0x7f80 : 0x7c00;  // bits of infinity
+
+  __device__ __forceinline__ void put(T a, T b) { w = __builtin_bit_cast(uint32_t, T2{a, b}); }
+  __device__ __forceinline__ T2 both() const { return __builtin_bit_cast(T2, w); }
+  // Running maximum of both halves' magnitudes (as bits, which order like the magnitudes); the float32 bits of it.
+  __device__ __forceinline__ static void most(uint32_t& m, Pair p, bool finite) {
+    u16x2 a = __builtin_bit_cast(u16x2, p.w & 0x7fff7fffu);
+    if (finite) {
+      a[0] = a[0] < kInf ? a[0] : (uint16_t)0;
+      a[1] = a[1] < kInf ? a[1] : (uint16_t)0;
+    }
+    m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), a));
+  }
+  __device__ __forceinline__ static uint32_t f32_bits(uint32_t m) {
+    const uint16_t x = (uint16_t)max(m & 0xffffu, m >> 16);
+    return __float_as_uint((float)__builtin_bit_cast(T, x));
+  }
+};
+
+template <>
+struct Pair<float> {
+  float a, b;
+  __device__ __forceinline__ void put(float x, float y) { a = x, b = y; }
+  __device__ __forceinline__ static void most(uint32_t& m, Pair p, bool finite) {
+    uint32_t x = __float_as_uint(p.a) & 0x7fffffffu, y = __float_as_uint(p.b) & 0x7fffffffu;
+    if (finite) {
+      x = x < 0x7f800000u ? x : 0u;
+      y = y < 0x7f800000u ? y : 0u;
+    }
+    m = max(m, max(x, y));
+  }
+  __device__ __forceinline__ static uint32_t f32_bits(uint32_t m) { return m; }
+};
+
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+
+// Codes of a pair's elements / scale, scale a power of two, in one rounding to nearest even, into half HI of `to`.
+template <bool HI, typename T>
+__device__ __forceinline__ i16x2 codes2(i16x2 to, Pair<T> p, float scale) {
+  if constexpr (__is_same(T, float)) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(to, p.a, p.b, scale, HI);
+  else if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(to, p.both(), scale, HI);
+  else return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(to, p.both(), scale, HI);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t codes4(Pair<T> p, Pair<T> q, float scale) {
+  i16x2 w = {0, 0};
+  w = codes2<false>(w, p, scale);
+  return __builtin_bit_cast(uint32_t, codes2<true>(w, q, scale));
+}
+
+// The values (code * scale, rounded to T once) of half HI's two codes.
+template <bool HI, typename T>
+__device__ __forceinline__ Pair<T> values2(uint32_t w, float scale) {
+  Pair<T> p;
+  if constexpr (__is_same(T, float)) {
+    const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, HI);
+    p.put(x[0], x[1]);
+  } else if constexpr (__is_same(T, _Float16)) {
+    p.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  } else {
+    p.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+  }
+  return p;
+}
+
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void load_pairs(const T* p, Pair<T> (&x)[N]) {
+  static_assert(sizeof(Pair<T>) == 2 * sizeof(T), "pairs are their elements' bytes");
+  if constexpr (ALIGNED) {
+    uint32_t w[N * sizeof(T) / 2];
+    load_words<N * 2 * sizeof(T)>(p, w);
+    __builtin_memcpy(x, w, sizeof(w));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i].put(p[2 * i], p[2 * i + 1]);
+  }
+}
+
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void store_pairs(T* p, const Pair<T> (&x)[N]) {
+  if constexpr (ALIGNED) {
+    uint32_t w[N * sizeof(T) / 2];
+    __builtin_memcpy(w, x, sizeof(w));
+    store_words<N * 2 * sizeof(T)>(p, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (__is_same(T, float)) p[2 * i] = x[i].a, p[2 * i + 1] = x[i].b;
+      else p[2 * i] = x[i].both()[0], p[2 * i + 1] = x[i].both()[1];
+    }
+  }
 }
 
 // The four codes of w at a scale 1/factor times as large: decoded, multiplied, rounded.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float factor) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-  return encode4(a[0] * factor, a[1] * factor, b[0] * factor, b[1] * factor);
+  int x = __builtin_amdgcn_cvt_pk_fp8_f32(a[0] * factor, a[1] * factor, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * factor, b[1] * factor, x, true);
 }
 
-__device__ __forceinline__ int new_exponent(int e, uint8_t* scale, bool keeps, int* old) {
-  *old = 0;
-  if (keeps) {
-    *old = min((int)*scale, 254);
-    e = max(e, *old);
-  }
-  return e;
+// V's part of a tile in one lane: kPairs pairs of channels from channel() on, and the tokens of kWords words of four:
+// all 32, or (head dim 64) those of the lane's half.
+template <int D>
+struct VPart {
+  static constexpr int kPairs = D == 256 ? 2 : 1, kWords = D == 64 ? 4 : 8;
+  int lane;
+  __device__ __forceinline__ int channel() const { return D == 64 ? 2 * (lane & 31) : lane * 2 * kPairs; }
+  __device__ __forceinline__ int word(int k) const { return D == 64 ? 4 * (lane >> 5) + k : k; }
+  // the first token of word k; tokens 8 (word & 3) + 4 (word >> 2) + 0..3
+  __device__ __forceinline__ int token(int k) const { return 8 * (word(k) & 3) + 4 * (word(k) >> 2); }
+};
+
+// Bytes of word w4 (tokens t .. t + 3) that belong to the tokens of the mask.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t mask, int t) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) b |= (mask >> (t + r) & 1u) ? 0xffu << (8 * r) : 0u;
+  return b;
 }
 
 template <typename T, int D, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvMove a) {
   const int lane = threadIdx.x & 63;
   Tile t;
-  if (!kv_tile_of(a, (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), &t)) return;
+  if (!kv_tile_of(a, blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), &t)) return;
   if (t.page < 0) return;
   const int64_t at = kv_tile(t.page, a.c.Hkv, t.h, D);
   const bool keeps = t.lo > 0 && t.q.first > 0;  // the block holds earlier tokens: places [0, lo)
   uint8_t* scale = (t.is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)t.page * a.c.Hkv + t.h;
+  const int held = min((int)*scale, 254), old = keeps ? held : 0;
+  // The page's exponent: of the largest magnitude among the new tokens (over all of them first; where that is no
+  // number, over the finite ones), and not below the one it has.
+  const auto exponent = [&](auto most) {
+    uint32_t m = wave_max(Pair<T>::f32_bits(most(false)));
+    if (m >= 0x7f800000u) m = wave_max(Pair<T>::f32_bits(most(true)));
+    return max(kv_exponent(m), old);
+  };
   if (!t.is_v) {
-    // 16 codes per lane and step: token and 16 channels, D/16 lanes across a token's row
+    // 16 codes per lane and step: a token's 16 channels, D/16 lanes across its row
     constexpr int N = D / 32, R = D / 16;
-    float x[N][16];
-    uint32_t m = 0;
+    Pair<T> x[N][8];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = i * 64 + lane, tok = id / R, d = id % R * 16;
-      if (tok >= t.lo && tok < t.hi) {
-        load_row<T, 16, ALIGNED>(reinterpret_cast<const T*>(a.k + (int64_t)(t.row + tok) * a.ldk) + t.h * D + d, x[i]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) m = max(m, amax_bits(x[i][j]));
-      }
+      for (int j = 0; j < 8; ++j) x[i][j].put((T)0.f, (T)0.f);
+      if (tok >= t.lo && tok < t.hi) load_pairs<T, 8, ALIGNED>(reinterpret_cast<const T*>(a.k + (int64_t)(t.row + tok) * a.ldk) + t.h * D + d, x[i]);
     }
-    int old;
-    const int e = new_exponent(kv_exponent(wave_max(m)), scale, keeps, &old);
-    const float factor = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e); e <= 254
+    const int e = exponent([&](bool finite) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) Pair<T>::most(m, x[i][j], finite);
+      return m;
+    });
+    const float step = __uint_as_float((uint32_t)e << 23);  // 2^(e - 127), as the conversions read it: exponent bits alone
     const bool grows = keeps && e > old;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -141,8 +251,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvMove a) {
       uint32_t w[4];
       if (tok >= t.lo && tok < t.hi) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = encode4(x[i][4 * j] * factor, x[i][4 * j + 1] * factor, x[i][4 * j + 2] * factor, x[i][4 * j + 3] * factor);
+        for (int j = 0; j < 4; ++j) w[j] = codes4(x[i][2 * j], x[i][2 * j + 1], step);
         store_words<16>(p, w);
       } else if (grows && tok < t.lo) {
         load_words<16>(p, w);
@@ -154,48 +263,64 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvMove a) {
     }
     if (lane == 0) *scale = (uint8_t)e;
   } else {
-    // D/64 channels per lane, all 32 tokens of each: the transposed tile needs no exchange between lanes
-    constexpr int E = D / 64;
-    float x[32][E];
-    uint32_t m = 0;
+    // A lane's tokens of its own channels: the transposed tile needs no exchange between lanes.
+    using Part = VPart<D>;
+    const Part part{lane};
+    constexpr int E = Part::kPairs, K = Part::kWords;
+    uint8_t* base = a.c.v + at + part.channel() * 32 + 4 * part.word(0);
+    const bool whole = t.lo == 0 && t.hi == 32;
+    uint32_t had[2 * E][K];
+    if (!whole) {
 #pragma unroll
-    for (int tok = 0; tok < 32; ++tok) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) x[tok][j] = 0.f;
-      if (tok >= t.lo && tok < t.hi) {
-        load_row<T, E, ALIGNED>(reinterpret_cast<const T*>(a.v + (int64_t)(t.row + tok) * a.ldv) + t.h * D + lane * E, x[tok]);
-#pragma unroll
-        for (int j = 0; j < E; ++j) m = max(m, amax_bits(x[tok][j]));
-      }
+      for (int c = 0; c < 2 * E; ++c) load_words<4 * K>(base + 32 * c, had[c]);
     }
-    int old;
-    const int e = new_exponent(kv_exponent(wave_max(m)), scale, keeps, &old);
-    const float factor = __uint_as_float((uint32_t)(254 - e) << 23);
-    const bool grows = keeps && e > old, whole = t.lo == 0 && t.hi == 32;
+    Pair<T> x[K][4][E];
+    const T* rows = reinterpret_cast<const T*>(a.v + (int64_t)t.row * a.ldv) + t.h * D + part.channel();
+    const int64_t ld = a.ldv / (int64_t)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = part.token(k) + r;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[k][r][j].put((T)0.f, (T)0.f);
+        if (tok >= t.lo && tok < t.hi) load_pairs<T, E, ALIGNED>(rows + tok * ld, x[k][r]);
+      }
+    const int e = exponent([&](bool finite) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < E; ++j) Pair<T>::most(m, x[k][r][j], finite);
+      return m;
+    });
+    const float step = __uint_as_float((uint32_t)e << 23);
+    const bool grows = keeps && e > old;
     const float f = __uint_as_float(kv_pow2_bits(old - e));
-    const uint32_t news = (t.hi == 32 ? 0xffffffffu : (1u << t.hi) - 1u) & ~((1u << t.lo) - 1u), olds = (1u << t.lo) - 1u;
+    const uint32_t olds = (1u << t.lo) - 1u, news = (t.hi == 32 ? 0xffffffffu : (1u << t.hi) - 1u) & ~olds;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      uint8_t* p = a.c.v + at + (lane * E + j) * 32;
-      uint32_t w[8], had[8];
-      if (!whole) load_words<32>(p, had);
+      uint32_t w[2][K];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int tok = 8 * (k & 3) + 4 * (k >> 2);  // the four tokens of word k
-        w[k] = encode4(x[tok][j] * factor, x[tok + 1][j] * factor, x[tok + 2][j] * factor, x[tok + 3][j] * factor);
+      for (int k = 0; k < K; ++k) {
+        const uint32_t lo = codes4(x[k][0][j], x[k][1][j], step), hi = codes4(x[k][2][j], x[k][3][j], step);
+        w[0][k] = __builtin_amdgcn_perm(hi, lo, 0x06040200u);  // four tokens of the pair's first channel
+        w[1][k] = __builtin_amdgcn_perm(hi, lo, 0x07050301u);
         if (!whole) {
-          uint32_t moved = had[k];
-          if (grows) moved = rescale4(had[k], f);
-          uint32_t mn = 0, mo = 0;  // bytes of new and of earlier tokens
+          const uint32_t mn = bytes_of(news, part.token(k)), mo = bytes_of(olds, part.token(k));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            mn |= (news >> (tok + r) & 1u) ? 0xffu << (8 * r) : 0u;
-            mo |= (olds >> (tok + r) & 1u) ? 0xffu << (8 * r) : 0u;
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t was = had[2 * j + c][k];
+            uint32_t moved = was;
+            if (grows) moved = rescale4(was, f);
+            w[c][k] = (w[c][k] & mn) | (moved & mo) | (was & ~(mn | mo));
           }
-          w[k] = (w[k] & mn) | (moved & mo) | (had[k] & ~(mn | mo));
         }
       }
-      store_words<32>(p, w);
+      store_words<4 * K>(base + 64 * j, w[0]);
+      store_words<4 * K>(base + 64 * j + 32, w[1]);
     }
     if (lane == 0) *scale = (uint8_t)e;
   }
@@ -205,12 +330,11 @@ template <typename T, int D, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvMove a) {
   const int lane = threadIdx.x & 63;
   Tile t;
-  if (!kv_tile_of(a, (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), &t)) return;
-  const bool none = t.page < 0;
+  if (!kv_tile_of(a, blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), &t)) return;
+  const bool none = t.page < 0;  // its codes are taken as zeros
   const int64_t page = none ? 0 : t.page, at = kv_tile(page, a.c.Hkv, t.h, D);
   const int e = (t.is_v ? a.c.v_scale : a.c.k_scale)[page * a.c.Hkv + t.h];
-  // 2^(e - 127), down to the subnormal 2^-127: exact products either way
-  const float factor = none ? 0.f : e == 0 ? 0x1p-127f : __uint_as_float((uint32_t)min(e, 254) << 23);
+  const float step = __uint_as_float((uint32_t)min(e, 254) << 23);  // 2^(e - 127), as the conversions read it
   if (!t.is_v) {
     constexpr int N = D / 32, R = D / 16;
 #pragma unroll
@@ -219,36 +343,44 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvMove a) {
       if (tok < t.lo || tok >= t.hi) continue;
       uint32_t w[4] = {0, 0, 0, 0};
       if (!none) load_words<16>(a.c.k + at + kv_k_place(tok, d), w);
-      float x[16];
+      Pair<T> x[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
-        x[4 * j] = lo[0] * factor, x[4 * j + 1] = lo[1] * factor, x[4 * j + 2] = hi[0] * factor, x[4 * j + 3] = hi[1] * factor;
+        x[2 * j] = values2<false, T>(w[j], step);
+        x[2 * j + 1] = values2<true, T>(w[j], step);
       }
-      store_row<T, 16, ALIGNED>(reinterpret_cast<T*>(a.k + (int64_t)(t.row + tok) * a.ldk) + t.h * D + d, x);
+      store_pairs<T, 8, ALIGNED>(reinterpret_cast<T*>(a.k + (int64_t)(t.row + tok) * a.ldk) + t.h * D + d, x);
     }
   } else {
-    constexpr int E = D / 64;
-    uint32_t w[E][8];
+    using Part = VPart<D>;
+    const Part part{lane};
+    constexpr int E = Part::kPairs, K = Part::kWords;
+    uint32_t w[2 * E][K];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
+    for (int c = 0; c < 2 * E; ++c) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[j][k] = 0;
-      if (!none) load_words<32>(a.c.v + at + (lane * E + j) * 32, w[j]);
+      for (int k = 0; k < K; ++k) w[c][k] = 0;
+      if (!none) load_words<4 * K>(a.c.v + at + (part.channel() + c) * 32 + 4 * part.word(0), w[c]);
     }
+    T* rows = reinterpret_cast<T*>(a.v + (int64_t)t.row * a.ldv) + t.h * D + part.channel();
+    const int64_t ld = a.ldv / (int64_t)sizeof(T);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float x[4][E];
+    for (int k = 0; k < K; ++k) {
+      Pair<T> x[4][E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j][k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j][k], true);
-        x[0][j] = lo[0] * factor, x[1][j] = lo[1] * factor, x[2][j] = hi[0] * factor, x[3][j] = hi[1] * factor;
+        // tokens 0, 1 and 2, 3 of the word, a channel pair of each in a half
+        const uint32_t lo = __builtin_amdgcn_perm(w[2 * j + 1][k], w[2 * j][k], 0x05010400u),
+                       hi = __builtin_amdgcn_perm(w[2 * j + 1][k], w[2 * j][k], 0x07030602u);
+        x[0][j] = values2<false, T>(lo, step);
+        x[1][j] = values2<true, T>(lo, step);
+        x[2][j] = values2<false, T>(hi, step);
+        x[3][j] = values2<true, T>(hi, step);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int tok = 8 * (k & 3) + 4 * (k >> 2) + r;
-        if (tok >= t.lo && tok < t.hi)
-          store_row<T, E, ALIGNED>(reinterpret_cast<T*>(a.v + (int64_t)(t.row + tok) * a.ldv) + t.h * D + lane * E, x[r]);
+        const int tok = part.token(k) + r;
+        if (tok >= t.lo && tok < t.hi) store_pairs<T, E, ALIGNED>(rows + tok * ld, x[r]);
       }
     }
   }
@@ -256,7 +388,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_kernel(KvMove a) {
 
 template <typename T, int D>
 hipError_t launch_d(const KvMove& a, bool write, bool aligned, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.tiles + kWaves - 1) / kWaves)), block(64 * kWaves);
+  const dim3 grid((a.tiles + kWaves - 1) / kWaves), block(64 * kWaves);
   if (write) {
     if (aligned) hipLaunchKernelGGL((kv_write_kernel<T, D, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((kv_write_kernel<T, D, false>), grid, block, 0, stream, a);
@@ -303,8 +435,10 @@ int kv_move(const sa_kv_rows_args* a, bool write, void* stream) {
   m.ldv = v.ld;
   const int64_t blocks = ((int64_t)a->seqs.max_rows + 30) / 32 + 1;  // r tokens touch at most (r + 62) / 32 blocks
   m.blocks = (int)blocks;
-  m.tiles = a->seqs.B * blocks * a->cache.Hkv * 2;
-  if (m.tiles > (int64_t)0x7fffffff * kWaves) return fail(SA_ERR_UNSUPPORTED, "%lld tiles in one call", (long long)m.tiles);
+  int64_t tiles = 0;  // 32-bit in the kernel: divisions of 64 bits took longer there than the tile itself
+  if (__builtin_mul_overflow(a->seqs.B * blocks, (int64_t)a->cache.Hkv * 2, &tiles) || tiles > 0x7fffffff)
+    return fail(SA_ERR_UNSUPPORTED, "B * max_rows / 32 * Hkv * 2 tiles of one call exceed 2^31");
+  m.tiles = (uint32_t)tiles;
   // every access of the aligned kernels is of 16 bytes or of a lane's channels at a multiple of them
   const bool aligned = (((uintptr_t)k.lo | (uintptr_t)v.lo | (uintptr_t)k.ld | (uintptr_t)v.ld) & 15) == 0;
   const hipError_t e = a->dtype == SA_DT_F32   ? launch_t<float>(m, write, aligned, (hipStream_t)stream)
