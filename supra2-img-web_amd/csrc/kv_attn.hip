@@ -318,7 +318,6 @@ __device__ __forceinline__ void store_o4(const KvAttnParams& a, const Work& w, i
 // 16x16x32 instructions: S^T of 16 keys x 16 rows leaves the keys 4 kq + i of a tile in lane (row, kq = lane >> 4), and the
 // two tiles of a page take its tokens in the order that makes those of one lane eight neighbouring codes of V:
 // tile u, place p: token 16 ((p >> 2) & 1) + 8 u + 4 (p >> 3) + (p & 3).
-constexpr int kSplitWaves = 4;
 
 __device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -497,12 +496,13 @@ __device__ __forceinline__ void step16(const Page16<D>& pg, Rows16<T, D> (&st)[N
   }
 }
 
-template <typename T, int D, int N>
-__global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_split_kernel(KvAttnParams a) {
+template <typename T, int D, int N, int W>
+__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void kv_attn_split_kernel(KvAttnParams a) {
   constexpr int ROWS = 16 * N, PAD = 20;
-  __shared__ __attribute__((aligned(16))) float lo[2][kSplitWaves][ROWS][PAD];
-  __shared__ float lm[kSplitWaves][ROWS], ll[kSplitWaves][ROWS];
-  __shared__ int lv[kSplitWaves];
+  static_assert(64 * W >= 4 * ROWS, "a thread for four channels of each row");
+  __shared__ __attribute__((aligned(16))) float lo[2][W][ROWS][PAD];
+  __shared__ float lm[W][ROWS], ll[W][ROWS];
+  __shared__ int lv[W];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int id = blockIdx.x;
@@ -510,19 +510,25 @@ __global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_sp
   id /= a.splits;
   const int group = id % a.groups;
   id /= a.groups;
+  // With all pages of a sequence in one workgroup, the first ones' ids need not wait for its length.
+  const int32_t* table = a.s.block_table + (int64_t)(id / a.c.Hkv) * a.s.max_blocks;
+  int32_t first = -1, next = -1;  // ids of the wave's first page, and of the page after the one being loaded
+  if (a.splits == 1) {
+    if (wave < a.s.max_blocks) first = table[wave];
+    if (wave + W < a.s.max_blocks) next = table[wave + W];
+  }
   Work w;
   if (!kv_work(a, ROWS, group, id % a.c.Hkv, id / a.c.Hkv, &w)) return;
   const int lo_block = (int)((int64_t)w.blocks * split / a.splits), hi_block = (int)((int64_t)w.blocks * (split + 1) / a.splits);
 
-  const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
   int blk = lo_block + wave;
-  Page16<D> pg[2];
-  int32_t next = -1;  // the id of the page after the one being loaded
-  if (blk < hi_block) {
-    const int32_t first = table[blk];
-    if (blk + kSplitWaves < hi_block) next = table[blk + kSplitWaves];
-    load_page<D>(a, w.hk, first, lane, pg[0]);
+  constexpr bool AHEAD = D <= 128;  // registers for two pages
+  Page16<D> pg[AHEAD ? 2 : 1];
+  if (a.splits > 1) {
+    first = blk < hi_block ? table[blk] : -1;
+    next = blk + W < hi_block ? table[blk + W] : -1;
   }
+  load_page<D>(a, w.hk, first, lane, pg[0]);
   Rows16<T, D> st[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) load_rows16<T, D>(a, w, w.row0 + 16 * n, lane, st[n]);
@@ -535,23 +541,35 @@ __global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_sp
   const int whole = min(hi_block, least / kKvBlock);
   const auto load_next = [&](int at, Page16<D>& p) {
     const int32_t now = next;
-    next = at + kSplitWaves < hi_block ? table[at + kSplitWaves] : -1;
+    next = at + W < hi_block ? table[at + W] : -1;
     load_page<D>(a, w.hk, now, lane, p);
   };
-  while (blk + kSplitWaves < whole) {
-    load_next(blk + kSplitWaves, pg[1]);
-    if (pg[0].ok) step16<T, D, N, false>(pg[0], st, mv, scale, lane, blk);
-    blk += kSplitWaves;
-    load_next(blk + kSplitWaves, pg[0]);  // past the last page: page 0, not used
-    if (pg[1].ok) step16<T, D, N, false>(pg[1], st, mv, scale, lane, blk);
-    blk += kSplitWaves;
+  if constexpr (!AHEAD) {
+    for (; blk < whole; blk += W) {
+      if (pg[0].ok) step16<T, D, N, false>(pg[0], st, mv, scale, lane, blk);
+      load_next(blk + W, pg[0]);
+    }
+    for (; blk < hi_block; blk += W) {
+      if (pg[0].ok) step16<T, D, N, true>(pg[0], st, mv, scale, lane, blk);
+      load_next(blk + W, pg[0]);
+    }
   }
-  while (blk < hi_block) {
-    const bool more = blk + kSplitWaves < hi_block;
-    if (more) load_next(blk + kSplitWaves, pg[1]);
-    if (pg[0].ok) step16<T, D, N, true>(pg[0], st, mv, scale, lane, blk);
-    pg[0] = pg[1];
-    blk += kSplitWaves;
+  if constexpr (AHEAD) {
+    while (blk + W < whole) {
+      load_next(blk + W, pg[1]);
+      if (pg[0].ok) step16<T, D, N, false>(pg[0], st, mv, scale, lane, blk);
+      blk += W;
+      load_next(blk + W, pg[0]);  // past the last page: page 0, not used
+      if (pg[1].ok) step16<T, D, N, false>(pg[1], st, mv, scale, lane, blk);
+      blk += W;
+    }
+    while (blk < hi_block) {
+      const bool more = blk + W < hi_block;
+      if (more) load_next(blk + W, pg[1]);
+      if (pg[0].ok) step16<T, D, N, true>(pg[0], st, mv, scale, lane, blk);
+      pg[0] = pg[1];
+      blk += W;
+    }
   }
 
   // ---- merge of the waves
@@ -569,22 +587,22 @@ __global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_sp
   float* rec = a.splits > 1 ? a.ws + record_at(a, w.b, w.hk, group, split, ROWS, D) : nullptr;
   int top_v = lv[0];
 #pragma unroll
-  for (int i = 1; i < kSplitWaves; ++i) top_v = max(top_v, lv[i]);
+  for (int i = 1; i < W; ++i) top_v = max(top_v, lv[i]);
   float mine[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     float m = lm[0][16 * n + r], total = 0.f;
 #pragma unroll
-    for (int i = 1; i < kSplitWaves; ++i) m = max_nan(m, lm[i][16 * n + r]);
+    for (int i = 1; i < W; ++i) m = max_nan(m, lm[i][16 * n + r]);
 #pragma unroll
-    for (int i = 0; i < kSplitWaves; ++i) total += ll[i][16 * n + r] * fast_exp2(lm[i][16 * n + r] - m);
+    for (int i = 0; i < W; ++i) total += ll[i][16 * n + r] * fast_exp2(lm[i][16 * n + r] - m);
     // rows that attended to nothing: sum 0, and zeros
     mine[n] = total == 0.f ? 0.f : fast_exp2(st[n].m - m) * __uint_as_float(kv_pow2_bits(mv - top_v)) / total;
     if (rec && wave == 0 && lane < 16) rec[ROWS * D + 16 * n + lane] = total == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(total);
   }
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) {
-    float(&half)[kSplitWaves][ROWS][PAD] = lo[e & 1];
+    float(&half)[W][ROWS][PAD] = lo[e & 1];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       f32x4 x;
@@ -598,7 +616,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, D <= 128 ? 2 : 1) void kv_attn_sp
     if (rr < ROWS) {
       f32x4 x = *reinterpret_cast<const f32x4*>(&half[0][rr][d]);
 #pragma unroll
-      for (int i = 1; i < kSplitWaves; ++i) x += *reinterpret_cast<const f32x4*>(&half[i][rr][d]);
+      for (int i = 1; i < W; ++i) x += *reinterpret_cast<const f32x4*>(&half[i][rr][d]);
       if (rec) *reinterpret_cast<f32x4*>(rec + rr * D + 16 * e + d) = x;
       else if (w.row0 + rr < w.rows) store_o4<T, D>(a, w, w.row0 + rr, 16 * e + d, x);
     }
@@ -787,6 +805,7 @@ __global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnParams a, int 
 }
 
 struct KvAttnPlan {
+  int waves;                       // of a workgroup
   int group_rows, groups, splits;  // of a row group; row groups of a sequence and key head; workgroups that share their keys
   bool many;                       // the kernel of many rows
   int64_t workgroups, ws_bytes;
@@ -803,8 +822,19 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
-  int64_t splits = (2 * kCUs + base - 1) / base;
-  if (splits > (blocks + 7) / 8) splits = (blocks + 7) / 8;
+  // Few rows, a quarter of the CUs to all of them with a workgroup each: eight waves to a workgroup, and the keys
+  // split (which costs the second launch) from 64 pages on. Against four waves and splits of eight pages: 16
+  // sequences of 2000 tokens at 8 key heads x 128 18.4 us (20.9), 32 of them 31.5 (35.5), 16 of 500 11.4 (13.0). With
+  // fewer workgroups the splits are quicker: one sequence of 2047 tokens 15.0 us in eight waves, 11.2 split.
+  p.waves = !p.many && base >= kCUs / 4 && base <= kCUs ? 8 : 4;
+  int64_t splits = 1;
+  if (p.waves == 4) {
+    splits = (2 * kCUs + base - 1) / base;
+    if (splits > (blocks + 7) / 8) splits = (blocks + 7) / 8;
+  } else if (blocks > 64) {
+    splits = (kCUs + base - 1) / base;
+    if (splits > (blocks + 31) / 32) splits = (blocks + 31) / 32;
+  }
   if (splits < 1) splits = 1;
   p.splits = (int)splits;
   p.workgroups = base * splits;
@@ -816,8 +846,12 @@ template <typename T, int D>
 hipError_t launch_kv_attn(const KvAttnParams& a, const KvAttnPlan& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.workgroups);
   if (p.many) hipLaunchKernelGGL((kv_attn_rows_kernel<T, D>), grid, dim3(64 * kRowWaves), 0, stream, a);
-  else if (p.group_rows == 16) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 1>), grid, dim3(64 * kSplitWaves), 0, stream, a);
-  else if constexpr (D <= 128) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 2>), grid, dim3(64 * kSplitWaves), 0, stream, a);
+  else if (p.group_rows == 16 && p.waves == 8) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 1, 8>), grid, dim3(64 * 8), 0, stream, a);
+  else if (p.group_rows == 16) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 1, 4>), grid, dim3(64 * 4), 0, stream, a);
+  else if constexpr (D <= 128) {
+    if (p.waves == 8) hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 2, 8>), grid, dim3(64 * 8), 0, stream, a);
+    else hipLaunchKernelGGL((kv_attn_split_kernel<T, D, 2, 4>), grid, dim3(64 * 4), 0, stream, a);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t most = (int64_t)a.s.max_rows * a.G;
@@ -847,7 +881,7 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   if (!isfinite(a->scale)) return fail(SA_ERR_INVALID, "scale must be finite");
   if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
   *p = KvAttnParams{};
-  *plan = KvAttnPlan{kRows, 0, 1, false, 0, 0};
+  *plan = KvAttnPlan{4, kRows, 0, 1, false, 0, 0};
   if (kv_nothing(a->seqs)) return SA_OK;
   const int size = kv_type_bytes(a->dtype);
   const int64_t width = (int64_t)a->H * a->cache.D;

@@ -23,7 +23,7 @@ namespace sa {
 
 namespace {
 
-constexpr int kWaves = 4;  // tiles per workgroup
+constexpr int kWaves = 2;  // tiles per workgroup
 
 struct KvMove {
   sa_kv_cache c;
@@ -270,10 +270,6 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvMove a) {
     uint8_t* base = a.c.v + at + part.channel() * 32 + 4 * part.word(0);
     const bool whole = t.lo == 0 && t.hi == 32;
     uint32_t had[2 * E][K];
-    if (!whole) {
-#pragma unroll
-      for (int c = 0; c < 2 * E; ++c) load_words<4 * K>(base + 32 * c, had[c]);
-    }
     Pair<T> x[K][4][E];
     const T* rows = reinterpret_cast<const T*>(a.v + (int64_t)t.row * a.ldv) + t.h * D + part.channel();
     const int64_t ld = a.ldv / (int64_t)sizeof(T);
@@ -299,6 +295,10 @@ __global__ __launch_bounds__(64 * kWaves) void kv_write_kernel(KvMove a) {
     const float step = __uint_as_float((uint32_t)e << 23);
     const bool grows = keeps && e > old;
     const float f = __uint_as_float(kv_pow2_bits(old - e));
+    if (!whole) {
+#pragma unroll
+      for (int c = 0; c < 2 * E; ++c) load_words<4 * K>(base + 32 * c, had[c]);
+    }
     const uint32_t olds = (1u << t.lo) - 1u, news = (t.hi == 32 ? 0xffffffffu : (1u << t.hi) - 1u) & ~olds;
 #pragma unroll
     for (int j = 0; j < E; ++j) {

@@ -259,14 +259,14 @@ def test_bounds_of_the_device_arrays(dev):
 
 # ---- attention
 
-def filled(rng, dev, lens, Hkv, D, spread=2, pages=None):
+def filled(rng, dev, lens, Hkv, D, spread=2, pages=None, extra=1):
     """A cache with random codes (NaN codes in every place that no sequence holds) and page scales 2^spread apart."""
     pages = pages or sum(-(-max(n, 0) // 32) for n in lens) + 2
     cache = ok.Cache(pages, Hkv, D, rng)
     cache.codes[cache.codes & 127 == 127] = 0x30
     cache.codes = np.where(rng.random(cache.codes.shape) < 0.5, cache.codes & 0x87 | 0x30, cache.codes & 0xBF)
     cache.exp = rng.integers(124 - spread, 125 + spread, cache.exp.shape).astype(np.uint8)
-    table = scattered_table(rng, lens, pages)
+    table = scattered_table(rng, lens, pages, extra)
     held = np.zeros((pages, ok.BLOCK), bool)
     for b, n in enumerate(lens):
         for j in range(max(n, 0)):
@@ -275,8 +275,8 @@ def filled(rng, dev, lens, Hkv, D, spread=2, pages=None):
     return cache, table
 
 
-def check_attention(dev, rng, rows, lens, H, Hkv, D, dtype, causal, T=None, spread=2, q_scale=1.0, max_len=0, uniform=False, **kw):
-    cache, table = filled(rng, dev, lens, Hkv, D, spread)
+def check_attention(dev, rng, rows, lens, H, Hkv, D, dtype, causal, T=None, spread=2, q_scale=1.0, max_len=0, uniform=False, extra=1, **kw):
+    cache, table = filled(rng, dev, lens, Hkv, D, spread, extra=extra)
     cached = Cached(dev, cache)
     T = T or sum(rows) + 1
     seqs = Sequences(dev, ok.Seqs(lens, table, T, max(rows), None if uniform else starts(rows)))
@@ -319,9 +319,15 @@ def test_attention_splits_and_their_merge(dev):
     """Few rows and many keys: the keys are split over workgroups; max_len shapes that and changes nothing else."""
     rng = np.random.default_rng(4)
     for dtype in TYPES:
-        assert check_attention(dev, rng, [1, 2], [2000, 40], 4, 2, 64, dtype, True) > 1
-    assert check_attention(dev, rng, [1], [900], 2, 1, 128, "BF16", True, max_len=900) > 1
-    assert check_attention(dev, rng, [1], [900], 2, 1, 128, "BF16", True, max_len=1) == 1
+        assert check_attention(dev, rng, [1, 2], [2500, 40], 4, 2, 64, dtype, True) > 1
+    assert check_attention(dev, rng, [1], [2500], 2, 1, 128, "BF16", True, max_len=2500) > 1
+    assert check_attention(dev, rng, [1], [2500], 2, 1, 128, "BF16", True, max_len=1) == 1
+    lens = [int(n) for n in rng.integers(1, 500, 20)]
+    assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, max_len=500) == 1  # eight waves a workgroup
+    assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, extra=70) > 1
+    assert check_attention(dev, rng, [3] * 20, [n + 3 for n in lens], 32, 4, 64, "F32", True, extra=70) > 1  # 32 rows
+    assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 128, "BF16", True, max_len=500) > 1  # four waves
+    assert check_attention(dev, rng, [100], [600], 2, 1, 64, "F16", True) > 1  # 128 rows each
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -491,8 +497,8 @@ def test_a_decoding_step_in_a_graph(dev):
     """The four calls captured once; replays with new inputs, lengths and pages in the same buffers equal eager calls."""
     rng = np.random.default_rng(22)
     B, H, Hkv, D, C = 3, 4, 1, 128, 64
-    table = rng.permutation(3 * 12).reshape(3, 12).astype(np.int32)
-    layer = Layer(dev, rng, B, H, Hkv, D, C, 36, 12, table, B, 1, 384)
+    table = rng.permutation(3 * 80).reshape(3, 80).astype(np.int32)
+    layer = Layer(dev, rng, B, H, Hkv, D, C, 240, 80, table, B, 1, 0)
     assert layer.attn.workspace_bytes > 0  # the keys are split: two launches and a workspace in the graph
     rows, lens = [1, 1, 1], [300, 33, 1]
     x = rng.standard_normal((B, C)).astype(np.float32)
