@@ -26,6 +26,7 @@
 #include <string.h>
 
 #include "supra_attn.h"
+#include "supra_kv.h"
 #include "supra_linear.h"
 #include "supra_vae.h"
 #include "supra_weights.h"
@@ -1142,6 +1143,183 @@ static napi_value js_conv3_pack(napi_env env, napi_callback_info info) {
   return undefined(env);
 }
 
+/* ---- norms with rotation, the 8-bit cache and attention over it (include/supra_kv.h) ---- */
+
+static int fits_i32(napi_env env, const int64_t* v, int n) {
+  for (int i = 0; i < n; ++i)
+    if (v[i] < INT32_MIN || v[i] > INT32_MAX) {
+      napi_throw_range_error(env, "SA_ERR_INVALID", "sizes and modes must fit in int32");
+      return 0;
+    }
+  return 1;
+}
+
+/* Bytes of a row element; 1 for a type the call refuses itself. */
+static int64_t row_bytes(int64_t dtype) { return dtype == SA_DT_F32 ? 4 : dtype == SA_DT_F16 || dtype == SA_DT_BF16 ? 2 : 1; }
+
+/* n rows of `width` elements from `off`, every ld (0: width), inside h */
+static int rows_in_bounds(napi_env env, const Handle* h, int64_t size, int64_t off, int64_t n, int64_t ld, int64_t width, const char* what) {
+  return n > 0 && in_bounds(env, h, 0, extent_bytes(size, off, 1, 0, n, ld ? ld : width, width), what);
+}
+
+/* (opts: dtype, T, H, Hkv, D, rotaryDim, pairs, norm, eps, ropeScale, q, k, qOff, kOff, ldq, ldk, qOut, kOut, qoOff, koOff,
+ * ldqo, ldko, qWeight, kWeight, invFreq (float64), positions) */
+static napi_value js_qk_norm_rope(napi_env env, napi_callback_info info) {
+  napi_value argv[1], v;
+  if (get_args(env, info, 1, argv)) return NULL;
+  sa_qk_rope_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  Handle *q, *k, *qo, *ko, *qw, *kw, *fr, *pos;
+  int64_t n[8];
+  double eps, rs;
+  napi_value o = argv[0];
+  if (prop_i64(env, o, "dtype", SA_DT_F32, &n[0]) || prop_i64(env, o, "T", -1, &n[1]) || prop_i64(env, o, "H", 0, &n[2]) ||
+      prop_i64(env, o, "Hkv", 0, &n[3]) || prop_i64(env, o, "D", -1, &n[4]) || prop_i64(env, o, "rotaryDim", 0, &n[5]) ||
+      prop_i64(env, o, "pairs", SA_ROPE_HALF, &n[6]) || prop_i64(env, o, "norm", SA_NORM_RMS, &n[7]) ||
+      prop_i64(env, o, "qOff", 0, &a.q_off) || prop_i64(env, o, "kOff", 0, &a.k_off) || prop_i64(env, o, "ldq", 0, &a.ldq) ||
+      prop_i64(env, o, "ldk", 0, &a.ldk) || prop_i64(env, o, "qoOff", 0, &a.qo_off) || prop_i64(env, o, "koOff", 0, &a.ko_off) ||
+      prop_i64(env, o, "ldqo", 0, &a.ldqo) || prop_i64(env, o, "ldko", 0, &a.ldko) || prop_buf(env, o, "q", &q) ||
+      prop_buf(env, o, "k", &k) || prop_buf(env, o, "qOut", &qo) || prop_buf(env, o, "kOut", &ko) || prop_buf(env, o, "qWeight", &qw) ||
+      prop_buf(env, o, "kWeight", &kw) || prop_buf(env, o, "invFreq", &fr) || prop_buf(env, o, "positions", &pos) ||
+      prop(env, o, "eps", &v) || get_f64(env, v, 1e-6, &eps, "eps") || prop(env, o, "ropeScale", &v) ||
+      get_f64(env, v, 1.0, &rs, "ropeScale") || !fits_i32(env, n, 8))
+    return NULL;
+  a.dtype = (int32_t)n[0], a.T = (int32_t)n[1], a.H = (int32_t)n[2], a.Hkv = (int32_t)n[3], a.D = (int32_t)n[4];
+  a.rotary_dim = (int32_t)n[5], a.pairs = (int32_t)n[6], a.norm = (int32_t)n[7];
+  a.eps = (float)eps, a.rope_scale = (float)rs;
+  a.q = ptr_of(q), a.k = ptr_of(k), a.q_out = ptr_of(qo), a.k_out = ptr_of(ko);
+  a.q_weight = (const float*)ptr_of(qw), a.k_weight = (const float*)ptr_of(kw);
+  a.inv_freq = (const double*)ptr_of(fr), a.positions = (const int32_t*)ptr_of(pos);
+  const int64_t size = row_bytes(a.dtype), wq = (int64_t)a.H * a.D, wk = (int64_t)a.Hkv * a.D;
+  if (rows_in_bounds(env, q, size, a.q_off, a.T, a.ldq, wq, "q") || rows_in_bounds(env, k, size, a.k_off, a.T, a.ldk, wk, "k") ||
+      rows_in_bounds(env, qo, size, a.qo_off, a.T, a.ldqo, wq, "qOut") || rows_in_bounds(env, ko, size, a.ko_off, a.T, a.ldko, wk, "kOut") ||
+      in_bounds(env, qw, 0, mul3(4, a.D, 1), "qWeight") || in_bounds(env, kw, 0, mul3(4, a.D, 1), "kWeight") ||
+      in_bounds(env, fr, 0, mul3(4, a.rotary_dim, 1), "invFreq") || in_bounds(env, pos, 0, mul3(4, a.T, 1), "positions") ||
+      ensure_stream(env))
+    return NULL;
+  if (throw_if(env, sa_qk_norm_rope(&a, g_stream))) return NULL;
+  return undefined(env);
+}
+
+/* opts: pages, Hkv, D, kCache, vCache, kScale, vScale; B, T, maxRows, maxBlocks, rowStart, seqLen, blockTable */
+static int fill_kv(napi_env env, napi_value o, sa_kv_cache* c, sa_kv_seqs* s) {
+  Handle *k, *v, *ks, *vs, *rs, *sl, *bt;
+  int64_t n[7];
+  memset(c, 0, sizeof *c);
+  memset(s, 0, sizeof *s);
+  if (prop_i64(env, o, "pages", -1, &n[0]) || prop_i64(env, o, "Hkv", -1, &n[1]) || prop_i64(env, o, "D", -1, &n[2]) ||
+      prop_i64(env, o, "B", -1, &n[3]) || prop_i64(env, o, "T", -1, &n[4]) || prop_i64(env, o, "maxRows", -1, &n[5]) ||
+      prop_i64(env, o, "maxBlocks", -1, &n[6]) || prop_buf(env, o, "kCache", &k) || prop_buf(env, o, "vCache", &v) ||
+      prop_buf(env, o, "kScale", &ks) || prop_buf(env, o, "vScale", &vs) || prop_buf(env, o, "rowStart", &rs) ||
+      prop_buf(env, o, "seqLen", &sl) || prop_buf(env, o, "blockTable", &bt) || !fits_i32(env, n, 7))
+    return 1;
+  c->pages = (int32_t)n[0], c->Hkv = (int32_t)n[1], c->D = (int32_t)n[2];
+  c->k = (uint8_t*)ptr_of(k), c->v = (uint8_t*)ptr_of(v), c->k_scale = (uint8_t*)ptr_of(ks), c->v_scale = (uint8_t*)ptr_of(vs);
+  s->B = (int32_t)n[3], s->T = (int32_t)n[4], s->max_rows = (int32_t)n[5], s->max_blocks = (int32_t)n[6];
+  s->row_start = (const int32_t*)ptr_of(rs), s->seq_len = (const int32_t*)ptr_of(sl), s->block_table = (const int32_t*)ptr_of(bt);
+  const int64_t bytes = sa_kv_cache_bytes(c->pages, c->Hkv, c->D);
+  if (bytes < 0) {
+    throw_last(env);
+    return 1;
+  }
+  return in_bounds(env, k, 0, bytes, "kCache") || in_bounds(env, v, 0, bytes, "vCache") ||
+         in_bounds(env, ks, 0, mul3(c->pages, c->Hkv, 1), "kScale") || in_bounds(env, vs, 0, mul3(c->pages, c->Hkv, 1), "vScale") ||
+         in_bounds(env, sl, 0, mul3(4, s->B, 1), "seqLen") || in_bounds(env, bt, 0, mul3(4, s->B, s->max_blocks), "blockTable") ||
+         in_bounds(env, rs, 0, mul3(4, (int64_t)s->B + 1, 1), "rowStart");
+}
+
+/* (opts: fill_kv's, dtype, k, v, kOff, vOff, ldk, ldv) */
+static napi_value kv_rows(napi_env env, napi_callback_info info, int (*call)(const sa_kv_rows_args*, void*)) {
+  napi_value argv[1];
+  if (get_args(env, info, 1, argv)) return NULL;
+  sa_kv_rows_args a;
+  memset(&a, 0, sizeof a);
+  a.struct_size = sizeof a;
+  Handle *k, *v;
+  int64_t dtype;
+  if (fill_kv(env, argv[0], &a.cache, &a.seqs) || prop_i64(env, argv[0], "dtype", SA_DT_F32, &dtype) || !fits_i32(env, &dtype, 1) ||
+      prop_buf(env, argv[0], "k", &k) || prop_buf(env, argv[0], "v", &v) || prop_i64(env, argv[0], "kOff", 0, &a.k_off) ||
+      prop_i64(env, argv[0], "vOff", 0, &a.v_off) || prop_i64(env, argv[0], "ldk", 0, &a.ldk) || prop_i64(env, argv[0], "ldv", 0, &a.ldv))
+    return NULL;
+  a.dtype = (int32_t)dtype;
+  a.k = ptr_of(k), a.v = ptr_of(v);
+  const int64_t size = row_bytes(dtype), width = (int64_t)a.cache.Hkv * a.cache.D;
+  if (rows_in_bounds(env, k, size, a.k_off, a.seqs.T, a.ldk, width, "k") || rows_in_bounds(env, v, size, a.v_off, a.seqs.T, a.ldv, width, "v") ||
+      ensure_stream(env))
+    return NULL;
+  if (throw_if(env, call(&a, g_stream))) return NULL;
+  return undefined(env);
+}
+static napi_value js_kv_write(napi_env env, napi_callback_info info) { return kv_rows(env, info, sa_kv_write); }
+static napi_value js_kv_read(napi_env env, napi_callback_info info) { return kv_rows(env, info, sa_kv_read); }
+
+/* (opts: fill_kv's, dtype, H, causal, scale, maxLen, q, out, qOff, oOff, ldq, ldo, workspace, workspaceBytes) */
+static int fill_kv_attn(napi_env env, napi_value o, sa_kv_attn_args* a) {
+  Handle *q, *out, *ws;
+  int64_t n[4];
+  double scale;
+  napi_value v;
+  memset(a, 0, sizeof *a);
+  a->struct_size = sizeof *a;
+  if (fill_kv(env, o, &a->cache, &a->seqs) || prop_i64(env, o, "dtype", SA_DT_F32, &n[0]) || prop_i64(env, o, "H", -1, &n[1]) ||
+      prop_i64(env, o, "causal", 0, &n[2]) || prop_i64(env, o, "maxLen", 0, &n[3]) || prop(env, o, "scale", &v) ||
+      get_f64(env, v, 1.0, &scale, "scale") || prop_buf(env, o, "q", &q) || prop_buf(env, o, "out", &out) ||
+      prop_buf(env, o, "workspace", &ws) || prop_i64(env, o, "qOff", 0, &a->q_off) || prop_i64(env, o, "oOff", 0, &a->o_off) ||
+      prop_i64(env, o, "ldq", 0, &a->ldq) || prop_i64(env, o, "ldo", 0, &a->ldo) ||
+      prop_i64(env, o, "workspaceBytes", 0, &a->workspace_bytes) || !fits_i32(env, n, 4))
+    return 1;
+  a->dtype = (int32_t)n[0], a->H = (int32_t)n[1], a->causal = (int32_t)n[2], a->max_len = (int32_t)n[3];
+  a->scale = (float)scale;
+  a->q = ptr_of(q), a->o = ptr_of(out), a->workspace = ptr_of(ws);
+  /* the call's own checks first (host only), so that a bad one reports its own error on any host */
+  int32_t rows, splits;
+  if (throw_if(env, sa_kv_attention_shape(a, &rows, &splits))) return 1;
+  const int64_t size = row_bytes(a->dtype), width = (int64_t)a->H * a->cache.D;
+  return rows_in_bounds(env, q, size, a->q_off, a->seqs.T, a->ldq, width, "q") ||
+         rows_in_bounds(env, out, size, a->o_off, a->seqs.T, a->ldo, width, "out") || in_bounds(env, ws, 0, a->workspace_bytes, "workspace");
+}
+
+static napi_value js_kv_attention(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (get_args(env, info, 1, argv)) return NULL;
+  sa_kv_attn_args a;
+  if (fill_kv_attn(env, argv[0], &a) || ensure_stream(env)) return NULL;
+  if (throw_if(env, sa_kv_attention(&a, g_stream))) return NULL;
+  return undefined(env);
+}
+
+static napi_value js_kv_attention_workspace_bytes(napi_env env, napi_callback_info info) {
+  napi_value argv[1], r;
+  if (get_args(env, info, 1, argv)) return NULL;
+  sa_kv_attn_args a;
+  if (fill_kv_attn(env, argv[0], &a)) return NULL;
+  const int64_t n = sa_kv_attention_workspace_bytes(&a);
+  if (n < 0) {
+    throw_last(env);
+    return NULL;
+  }
+  NAPI_CALL(env, napi_create_int64(env, n, &r));
+  return r;
+}
+
+/* (pages, Hkv, D) */
+static napi_value js_kv_cache_bytes(napi_env env, napi_callback_info info) {
+  napi_value argv[3], r;
+  int64_t n[3];
+  if (get_args(env, info, 3, argv)) return NULL;
+  if (get_i64(env, argv[0], -1, &n[0], "pages") || get_i64(env, argv[1], -1, &n[1], "Hkv") || get_i64(env, argv[2], -1, &n[2], "D") ||
+      !fits_i32(env, n, 3))
+    return NULL;
+  const int64_t bytes = sa_kv_cache_bytes((int32_t)n[0], (int32_t)n[1], (int32_t)n[2]);
+  if (bytes < 0) {
+    throw_last(env);
+    return NULL;
+  }
+  NAPI_CALL(env, napi_create_int64(env, bytes, &r));
+  return r;
+}
+
 static napi_value init(napi_env env, napi_value exports) {
   const napi_property_descriptor props[] = {
       {"attention", NULL, js_attention, NULL, NULL, NULL, napi_enumerable, NULL},
@@ -1180,6 +1358,12 @@ static napi_value init(napi_env env, napi_value exports) {
       {"toF32", NULL, js_to_f32, NULL, NULL, NULL, napi_enumerable, NULL},
       {"rowsF32", NULL, js_rows_f32, NULL, NULL, NULL, napi_enumerable, NULL},
       {"conv3Pack", NULL, js_conv3_pack, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"qkNormRope", NULL, js_qk_norm_rope, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"kvCacheBytes", NULL, js_kv_cache_bytes, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"kvWrite", NULL, js_kv_write, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"kvRead", NULL, js_kv_read, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"kvAttention", NULL, js_kv_attention, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"kvAttentionWorkspaceBytes", NULL, js_kv_attention_workspace_bytes, NULL, NULL, NULL, napi_enumerable, NULL},
   };
   NAPI_CALL(env, napi_define_properties(env, exports, sizeof props / sizeof props[0], props));
   napi_value c;
@@ -1192,6 +1376,11 @@ static napi_value init(napi_env env, napi_value exports) {
   CONST("SA_MASK_NONE", SA_MASK_NONE)
   CONST("SA_MASK_KEY_LEN", SA_MASK_KEY_LEN)
   CONST("SA_MASK_KEY_MASK", SA_MASK_KEY_MASK)
+  CONST("SA_NORM_NONE", SA_NORM_NONE)
+  CONST("SA_NORM_RMS", SA_NORM_RMS)
+  CONST("SA_ROPE_HALF", SA_ROPE_HALF)
+  CONST("SA_ROPE_NEAR", SA_ROPE_NEAR)
+  CONST("SA_KV_BLOCK", SA_KV_BLOCK)
   CONST("SA_DT_F32", SA_DT_F32)
   CONST("SA_DT_F16", SA_DT_F16)
   CONST("SA_DT_BF16", SA_DT_BF16)

@@ -12,11 +12,13 @@
 //
 //   selfAttention(gpu, qkv, B, opts)     -> Tensor [B*T, dim]
 //   packContexts(gpu, kvs, lens, opts)   -> { kv, keyLen, lens, Lmax, B, release() }
-//   crossAttention(gpu, q, ctx, opts)    -> Tensor [B*T, dim]
+//   cacheContexts(gpu, kvs, lens, opts)  -> a context in the 8-bit cache: a quarter of the memory, for runs that keep many
+//   crossAttention(gpu, q, ctx, opts)    -> Tensor [B*T, dim], for either kind of context
 // opts: { tokens = 256, dim = 576, heads = 9, out } (the DiT config of app/models/dit.js).
 "use strict";
 
 var ops = require("./ops");
+var kvc = require("./kv_cache");
 
 function cfg(opts) {
   var o = opts || {};
@@ -70,9 +72,48 @@ function packContexts(gpu, kvs, lens, opts) {
   };
 }
 
-// Cross-attention of all B samples to their packed contexts: equals the dit.js:180-185 loop.
+// The same contexts quantised into a cache of their own (one scale for K and one for V of 32 tokens and head), each
+// sample's pages one after another. K and V keep 4 significant bits: the result is that of the rounded contexts.
+function cacheContexts(gpu, kvs, lens, opts) {
+  var c = cfg(opts);
+  var B = kvs.length;
+  if (lens.length !== B) throw new RangeError("one length per context");
+  var total = 0, pages = 0, blocks = [], row = 2 * c.dim * 4;
+  for (var b = 0; b < B; b++) {
+    if (!(lens[b] >= 0)) throw new RangeError("context lengths must be >= 0");
+    if (lens[b] > 0 && (!kvs[b] || !kvs[b].buf)) {
+      var e = new Error("context " + b + " is a released or invalid Tensor");
+      e.code = "SA_ERR_INVALID";
+      throw e;
+    }
+    total += lens[b];
+    blocks.push([]);
+    for (var n = 0; n < lens[b]; n += kvc.BLOCK) blocks[b].push(pages++);
+  }
+  var cache = new kvc.KvCache(gpu, { pages: Math.max(1, pages), Hkv: c.H, D: c.D });
+  var rows = gpu.empty([Math.max(1, total), 2 * c.dim]), at = 0;
+  var written = kvc.sequences(gpu, { lens: lens, blocks: blocks });
+  for (b = 0; b < B; b++) {
+    if (lens[b] === 0) continue;
+    gpu.op({ name: "copy", flops: 0 }, function () {
+      gpu.native.copy(rows.buf, at * row, kvs[b].buf, 0, lens[b] * row);
+    });
+    at += lens[b];
+  }
+  kvc.write(gpu, cache, written, { k: rows, v: rows, vOff: c.dim, ldk: 2 * c.dim, ldv: 2 * c.dim });
+  rows.release();  // stream-ordered pool reuse
+  written.release();
+  var queries = kvc.sequences(gpu, { lens: lens, rows: kvs.map(function () { return c.T; }), blocks: blocks });
+  return {
+    cache: cache, seqs: queries, lens: Int32Array.from(lens), B: B,
+    release: function () { cache.release(); queries.release(); },
+  };
+}
+
+// Cross-attention of all B samples to their packed or cached contexts: equals the dit.js:180-185 loop.
 function crossAttention(gpu, q, ctx, opts) {
   var c = cfg(opts);
+  if (ctx.cache) return kvc.attention(gpu, ctx.cache, ctx.seqs, { q: q, H: c.H, out: c.out });
   var ldkv = 2 * c.dim;
   return ops.attention(gpu, {
     B: ctx.B, q: q, k: ctx.kv, v: ctx.kv, Lq: c.T, Lk: ctx.Lmax, H: c.H, D: c.D, ldq: c.dim, ldk: ldkv, ldv: ldkv,
@@ -82,4 +123,4 @@ function crossAttention(gpu, q, ctx, opts) {
   });
 }
 
-module.exports = { selfAttention: selfAttention, packContexts: packContexts, crossAttention: crossAttention };
+module.exports = { selfAttention: selfAttention, packContexts: packContexts, cacheContexts: cacheContexts, crossAttention: crossAttention };
