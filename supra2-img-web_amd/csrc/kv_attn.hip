@@ -117,11 +117,29 @@ __device__ __forceinline__ float q_factor(const KvAttnParams& a, uint32_t m, int
   return copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
 }
 
-// Q's operand for one 32-row group: lane (row = lane & 31, half): elements 32c + 16 half .. + 16 of each chunk c.
+// Q's operand for one 32-row group. float16 terms, one for float16 rows and two for float32: lane (row = lane & 31, half) has elements 32 c +
+// 16 half .. + 16 of each chunk c.
 template <typename T, int D>
 struct QTile {
   f16x8 t[D / 32][2][kTerms<T>];
   int exponent;  // the row's elements are 2^exponent times the operand's
+};
+
+// bfloat16 rows, e4m3 terms for the scaled 32x32x64 products, in the same places: word 0..3 of operand i chunk 2 i, 4..7 chunk
+// 2 i + 1, each with the scale of the row's 32 elements of that chunk, which lanes of half 0 and half 1 give (the
+// instruction takes the scale of both halves' first 16 bytes from the one and of their last 16 from the other). K's codes
+// are the other operand as they are, its page's exponent their scale. A bfloat16 element has 8 bits, two terms of 4:
+// against one float16 term K needs no conversion (4 x 2048 rows over 4096 keys at 32 heads x 128: 598 us -> 560). A
+// float16 element would take three (16 heads x 64: 130 -> 132) and keeps the float16 products.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+constexpr int kTerms8 = 2;
+template <typename T>
+constexpr bool kCodes = __is_same(T, __bf16);  // rows that the kernel of many rows takes in e4m3 terms
+
+template <typename T, int D>
+struct QCodes {
+  i32x8 t[D / 64][kTerms8];
+  int e[D / 64];  // exponent byte of the first term's chunk 2 i + half; the second's is 4 less
 };
 
 // Rows of 32 in one wave, as memory has them and as the operands want them. Memory: a chunk of 32 channels of a row is
@@ -139,13 +157,12 @@ __device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
   return (int64_t)((uint64_t)(uint32_t)__shfl((int)(x >> 32), lane) << 32 | (uint32_t)__shfl((int)x, lane));
 }
 
+// A wave's 32 rows of q in float32: lane (row, half): channels 32 c + 16 half on.
 template <typename T, int D>
-__device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int lane, QTile<T, D>& q, char* lds) {
+__device__ __forceinline__ void load_rows32(const KvAttnParams& a, const Work& w, int lane, char* lds, float (&x)[D / 32][16]) {
   constexpr int C = D / 32;
   const int half = lane >> 5;
   const int64_t place = row_place(a, w, w.row0 + (lane & 31), a.ldq, D * (int)sizeof(T));
-  float x[C][16];
-  uint32_t m = 0;
   if (a.aligned_q) {
     constexpr int PARTS = 2 * (int)sizeof(T), STEPS = PARTS / 2, STRIDE = 16 * PARTS + 16;  // of a chunk's row; wave steps of 64
     static_assert(32 * STRIDE <= kRowsLds, "the chunk fits");
@@ -175,23 +192,69 @@ __device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[c][i] = 0.f;
+      for (int j = 0; j < 16; ++j) x[c][j] = 0.f;
       if (place >= 0) load_row<T, 16, false>(reinterpret_cast<const T*>(a.q + place) + 32 * c + 16 * half, x[c]);
     }
   }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int lane, QTile<T, D>& q, char* lds) {
+  float x[D / 32][16];
+  load_rows32<T, D>(a, w, lane, lds, x);
+  uint32_t m = 0;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < D / 32; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[c][i]) & 0x7fffffffu);
   auto sw = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   m = max(sw[0], sw[1]);
   const float factor = q_factor(a, m, q.exponent);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
+  for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[c][i] *= factor;
     split8<kTerms<T>>(x[c], q.t[c][0]);
     split8<kTerms<T>>(x[c] + 8, q.t[c][1]);
+  }
+}
+
+// The second term is the rest of the first, at a 16th of its scale: with the first scale the smallest that keeps the
+// largest element within 448, the rest is at most half a step of 32, 16 = 256 sixteenths. Elements down to 2^-14 of the
+// largest of their 32 are exact, smaller ones within 2^-22 of it.
+template <typename T, int D>
+__device__ __forceinline__ void load_q(const KvAttnParams& a, const Work& w, int lane, QCodes<T, D>& q, char* lds) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  float x[D / 32][16];
+  load_rows32<T, D>(a, w, lane, lds, x);
+  const uint32_t sign = __float_as_uint(a.scale_log2) & 0x80000000u;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      x[c][j] = __uint_as_float(__float_as_uint(x[c][j]) ^ sign);
+      m = max(m, __float_as_uint(x[c][j]) & 0x7fffffffu);
+    }
+    auto sw = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    const int e = max(kv_exponent(max(sw[0], sw[1])), 4 * (kTerms8 - 1));
+    if ((c & 1) == lane >> 5) q.e[c / 2] = e;
+#pragma unroll
+    for (int t = 0; t < kTerms8; ++t) {
+      const float step = __uint_as_float((uint32_t)(e - 4 * t) << 23);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        i16x2 w2 = {0, 0};
+        w2 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w2, x[c][j], x[c][j + 1], step, false);
+        w2 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w2, x[c][j + 2], x[c][j + 3], step, true);
+        const int word = __builtin_bit_cast(int, w2);
+        q.t[c / 2][t][4 * (c & 1) + j / 4] = word;
+        if (t + 1 < kTerms8) {
+          const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, step, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, step, true);
+          x[c][j] -= lo[0], x[c][j + 1] -= lo[1], x[c][j + 2] -= hi[0], x[c][j + 3] -= hi[1];
+        }
+      }
+    }
   }
 }
 
@@ -212,13 +275,44 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 }
 __device__ __forceinline__ uint32_t ones_at_nan(uint32_t w) { return (nan_bytes(w) >> 7) * 0x38u; }  // 0x38: the code of 1
 
+// S^T of a page, and the factor that makes it log2 units. k(c): the lane's 16 bytes of KiB c of the K tile.
+template <typename T, int D, typename K>
+__device__ __forceinline__ f32x16 scores(const QTile<T, D>& q, const K& k, int ke, float scale_log2, float& f) {
+  f32x16 s = zero16();
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    const u32x4 x = k(c);
+    const f16x8 k0 = half8(x[0], x[1], 1.f), k1 = half8(x[2], x[3], 1.f);
+#pragma unroll
+    for (int t = kTerms<T> - 1; t >= 0; --t) {
+      s = mfma(k0, q.t[c][0][t], s);
+      s = mfma(k1, q.t[c][1][t], s);
+    }
+  }
+  f = ldexpf(scale_log2, q.exponent + ke - 127);  // >= 0
+  return s;
+}
+
+template <typename T, int D, typename K>
+__device__ __forceinline__ f32x16 scores(const QCodes<T, D>& q, const K& k, int ke, float scale_log2, float& f) {
+  f32x16 s = zero16();
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const u32x4 lo = k(2 * i), hi = k(2 * i + 1);
+    const i32x8 x = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+#pragma unroll
+    for (int t = kTerms8 - 1; t >= 0; --t) s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, q.t[i][t], s, 0, 0, 0, ke, 0, q.e[i] - 4 * t);
+  }
+  f = scale_log2;
+  return s;
+}
+
 // One page of 32 keys. k(c), v(c): the lane's 16 bytes of KiB c of its K and V tiles. MASKED: of the page's keys each row
 // attends to the first `limit` (its own).
-template <typename T, int D, bool MASKED, typename LoadK, typename LoadV>
-__device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const LoadK& k, const LoadV& v, int ke, int ve,
-                                     float scale_log2, int lane, int limit) {
+template <typename T, int D, bool MASKED, typename Q, typename LoadK, typename LoadV>
+__device__ __forceinline__ void step(const Q& q, State<D>& st, const LoadK& k, const LoadV& v, int ke, int ve, float scale_log2,
+                                     int lane, int limit) {
   constexpr int NT = kTerms<T>;
-  f32x16 s = zero16();
   // Where registers allow, the whole page is on its way before the first product (the compiler would fetch V's part
   // after the exponentials: 630 us against 619 for 4 x 2048 rows over 4096 keys at 32 heads x 128).
   constexpr bool EARLY = D <= 128;
@@ -230,17 +324,8 @@ __device__ __forceinline__ void step(const QTile<T, D>& q, State<D>& st, const L
     for (int c = 0; c < D / 32; ++c) vr[c] = v(c);
     __builtin_amdgcn_sched_barrier(0);
   }
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    const u32x4 x = EARLY ? kr[c] : k(c);
-    const f16x8 k0 = half8(x[0], x[1], 1.f), k1 = half8(x[2], x[3], 1.f);
-#pragma unroll
-    for (int t = NT - 1; t >= 0; --t) {
-      s = mfma(k0, q.t[c][0][t], s);
-      s = mfma(k1, q.t[c][1][t], s);
-    }
-  }
-  const float f = ldexpf(scale_log2, q.exponent + ke - 127);  // >= 0
+  float f;
+  f32x16 s = scores(q, [&](int c) { return EARLY ? kr[c] : k(c); }, ke, scale_log2, f);
   const int half = lane >> 5;
   float top;
   if constexpr (MASKED) {
@@ -700,7 +785,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
   const bool on = kv_work(a, kRows, block4 * kRowWaves + wave, w.hk, w.b, &w);  // waves past the last rows only load
   const int lo_block = (int)((int64_t)all.blocks * split / a.splits), hi_block = (int)((int64_t)all.blocks * (split + 1) / a.splits);
 
-  QTile<T, D> q;
+  std::conditional_t<kCodes<T>, QCodes<T, D>, QTile<T, D>> q;
   State<D> st;
   char* mine = shared + wave * kRowsLds;
   if (on) load_q<T, D>(a, w, lane, q, mine);

@@ -342,7 +342,8 @@ def test_attention_forms(dev, dtype):
     check_attention(dev, rng, [2, 40], [100, 70], 2, 1, 64, dtype, True, spread=8, q_scale=2.0 ** -6)
 
 
-def test_attention_nan_where_it_is_not_attended(dev):
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_nan_where_it_is_not_attended(dev, dtype):
     """NaN codes at tokens behind a row's position leave the row alone, and reach the rows that attend to them."""
     rng = np.random.default_rng(8)
     for D in (64, 128, 256):
@@ -351,13 +352,46 @@ def test_attention_nan_where_it_is_not_attended(dev):
         cache.codes[0, table[0, 2], 0, 2, 5] = 0xFF    # K of token 66
         cached = Cached(dev, cache)
         seqs = Sequences(dev, ok.Seqs([70], table, 70, 70, [0, 70]))
-        q = ok.to_type(rng.standard_normal((70, 2 * D)), "F32")
-        got, ro, _ = attend(dev, cached, seqs, q, 2, "F32", D ** -0.5, True)
-        o, size, reach, count, mine = cache.attention(seqs.oracle, q.astype(np.float64).reshape(70, 2, D), D ** -0.5, True)
+        q = ok.to_type(rng.standard_normal((70, 2 * D)), dtype)
+        got, ro, _ = attend(dev, cached, seqs, q, 2, dtype, D ** -0.5, True)
+        o, size, reach, count, mine = cache.attention(seqs.oracle, ok.values(q, dtype).reshape(70, 2, D), D ** -0.5, True)
         assert np.isfinite(o[:52]).all() and np.isnan(o[52:, :, 3]).all() and np.isfinite(o[52:66, :, 4]).all() and np.isnan(o[66:]).all()
-        near(got, o, ok.attention_tolerance(o, size, reach, count, D, "F32"), f"D {D}")
+        near(got, o, ok.attention_tolerance(o, size, reach, count, D, dtype), f"D {D}")
         for x in (cached, seqs, ro):
             x.release()
+        # a few rows, in tiles of 16
+        seqs = Sequences(dev, ok.Seqs([70], table, 20, 20, [0, 20]))
+        cached = Cached(dev, cache)
+        got, ro, _ = attend(dev, cached, seqs, q[:20, :D], 1, dtype, D ** -0.5, True)
+        o, size, reach, count, mine = cache.attention(seqs.oracle, ok.values(q[:20, :D], dtype).reshape(20, 1, D), D ** -0.5, True)
+        assert np.isfinite(o[:2]).all() and np.isnan(o[2:, :, 3]).all() and np.isfinite(o[2:16, :, 4]).all() and np.isnan(o[16:]).all()
+        near(got, o, ok.attention_tolerance(o, size, reach, count, D, dtype), f"D {D}, 20 rows")
+        for x in (cached, seqs, ro):
+            x.release()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_queries_of_every_size(dev, dtype):
+    """Elements of a row from 2^-9 to 2^5 of each other, rows of zeros, infinities and NaN, a negative scale."""
+    rng = np.random.default_rng(13)
+    D, n, H = 128, 90, 2
+    cache, table = filled(rng, dev, [100], 1, D)
+    cached = Cached(dev, cache)
+    for rows in (n, 7):
+        x = rng.standard_normal((rows, H * D)) * np.exp2(rng.integers(-9, 6, (rows, H * D))) / 4
+        x[1], x[2, 5], x[3, D + 7], x[4, 3] = 0, np.inf, np.nan, -np.inf
+        q = ok.to_type(x, dtype)
+        seqs = Sequences(dev, ok.Seqs([100], table, rows, rows))
+        for scale in (0.0625, -0.0625, 0.0):
+            got, ro, _ = attend(dev, cached, seqs, q, H, dtype, scale, True)
+            qv = ok.values(q, dtype).reshape(rows, H, D)
+            with np.errstate(invalid="ignore"):
+                o, size, reach, count, _ = cache.attention(seqs.oracle, qv, scale, True)
+            o[~np.isfinite(qv).all(-1)] = np.nan  # inf - inf, or 0 * inf, in the scores
+            near(got, o, ok.attention_tolerance(o, size, reach, count, D, dtype), f"rows {rows} scale {scale}")
+            ro.release()
+        seqs.release()
+    cached.release()
 
 
 def test_pages_beyond_32_bit_offsets(dev):
