@@ -1052,7 +1052,8 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   const int G = a->H / a->cache.Hkv;
   if ((int64_t)a->seqs.max_rows * G > (1 << 30)) return fail(SA_ERR_UNSUPPORTED, "%d rows of %d heads in one sequence", a->seqs.max_rows, G);
   *plan = kv_attn_plan(a);
-  if (plan->workgroups > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%lld workgroups in one call", (long long)plan->workgroups);
+  if (plan->workgroups > kKvMaxThreads / (64 * plan->waves))
+    return fail(SA_ERR_UNSUPPORTED, "%lld workgroups: more than one launch takes", (long long)plan->workgroups);
   p->c = a->cache;
   p->s = a->seqs;
   p->q = q.lo;

@@ -436,8 +436,8 @@ int kv_move(const sa_kv_rows_args* a, bool write, void* stream) {
   const int64_t blocks = ((int64_t)a->seqs.max_rows + 30) / 32 + 1;  // r tokens touch at most (r + 62) / 32 blocks
   m.blocks = (int)blocks;
   int64_t tiles = 0;  // 32-bit in the kernel: divisions of 64 bits took longer there than the tile itself
-  if (__builtin_mul_overflow(a->seqs.B * blocks, (int64_t)a->cache.Hkv * 2, &tiles) || tiles > 0x7fffffff)
-    return fail(SA_ERR_UNSUPPORTED, "B * max_rows / 32 * Hkv * 2 tiles of one call exceed 2^31");
+  if (__builtin_mul_overflow(a->seqs.B * blocks, (int64_t)a->cache.Hkv * 2, &tiles) || tiles > kKvMaxThreads / 64 - kWaves)
+    return fail(SA_ERR_UNSUPPORTED, "2 * Hkv tiles of each 32 rows of each sequence: more than 2^26 in one call");
   m.tiles = (uint32_t)tiles;
   // every access of the aligned kernels is of 16 bytes or of a lane's channels at a multiple of them
   const bool aligned = (((uintptr_t)k.lo | (uintptr_t)v.lo | (uintptr_t)k.ld | (uintptr_t)v.ld) & 15) == 0;

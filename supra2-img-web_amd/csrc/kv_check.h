@@ -9,6 +9,7 @@
 namespace sa {
 
 constexpr int64_t kKvMaxStride = (int64_t)1 << 40;
+constexpr int64_t kKvMaxThreads = ((int64_t)1 << 32) - 1;  // of one launch
 
 inline int kv_type_bytes(int32_t dtype) { return dtype == SA_DT_F32 ? 4 : dtype == SA_DT_F16 || dtype == SA_DT_BF16 ? 2 : 0; }
 

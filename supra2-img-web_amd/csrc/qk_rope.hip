@@ -304,7 +304,7 @@ extern "C" int sa_qk_norm_rope(const sa_qk_rope_args* args, void* stream) {
   p.per_wave = per * step;
   p.runs = (steps + per - 1) / per;
   const int64_t groups = ((int64_t)p.T * p.runs + sa::kRopeWaves - 1) / sa::kRopeWaves;
-  if (groups > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%lld workgroups in one call", (long long)groups);
+  if (groups > sa::kKvMaxThreads / (64 * sa::kRopeWaves)) return fail(SA_ERR_UNSUPPORTED, "T = %d tokens: more than one launch takes", p.T);
   const bool near = args->pairs == SA_ROPE_NEAR;
   const hipStream_t s = (hipStream_t)stream;
   const unsigned grid = (unsigned)groups;

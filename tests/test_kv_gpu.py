@@ -394,6 +394,38 @@ def test_attention_queries_of_every_size(dev, dtype):
     cached.release()
 
 
+def test_without_pages_and_with_shared_ones(dev):
+    """No column in the block table: rows of zeros. One page in the tables of 70000 sequences: the same row for each."""
+    rng = np.random.default_rng(17)
+    D = 64
+    cache, _ = filled(rng, dev, [32], 1, D)
+    cache.codes[cache.codes & 127 == 127] = 0x30
+    cached = Cached(dev, cache)
+    q = ok.to_type(rng.standard_normal((3, D)), "BF16")
+    for rows in (1, 3):
+        none = Sequences(dev, ok.Seqs([50] * (3 // rows), np.zeros((3 // rows, 0), np.int32), 3, rows))
+        none.desc.max_blocks = 0
+        got, ro, _ = attend(dev, cached, none, q, 1, "BF16", 0.125, False)
+        assert (got == 0).all()
+        gk, gv, rk, rv = read_call(dev, cached, none, "BF16")
+        assert (gk == 0).all() and (gv == 0).all()
+        write_call(dev, cached, none, q, q, "BF16")  # nowhere to
+        same_cache(cached.now(), cache)
+        for x in (none, ro, rk, rv):
+            x.release()
+    B = 70000
+    many = Sequences(dev, ok.Seqs([20] * B, np.zeros((B, 1), np.int32), B, 1))
+    got, ro, _ = attend(dev, cached, many, np.repeat(q[:1], B, 0), 1, "BF16", 0.125, True)
+    assert (got == got[:1]).all()
+    o, size, reach, count, _ = cache.attention(ok.Seqs([20], [[0]], 1, 1), ok.values(q[:1], "BF16").reshape(1, 1, D), 0.125, True)
+    near(got[:1], o, ok.attention_tolerance(o, size, reach, count, D, "BF16"))
+    gk, gv, rk, rv = read_call(dev, cached, many, "F32")
+    wk, wv, _ = cache.read(ok.Seqs([20], [[0]], 1, 1), 1)
+    assert (gk == wk).all() and (gv == wv).all()
+    for x in (cached, many, ro, rk, rv):
+        x.release()
+
+
 def test_pages_beyond_32_bit_offsets(dev):
     """A cache of more than 4 GiB for K and for V: its last pages are written, read and attended to."""
     rng = np.random.default_rng(11)

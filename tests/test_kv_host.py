@@ -243,6 +243,19 @@ def test_refusals_of_norm_rope(status, over):
     assert lib.sa_qk_norm_rope(ctypes.byref(rope_args(**over)), None) == status and lib.sa_last_error()
 
 
+@no_device
+def test_calls_that_one_launch_cannot_hold():
+    lib = _lib.load()
+    huge = dict(B=1 << 20, T=1 << 30, max_rows=1 << 10, max_blocks=1 << 10)
+    apart = dict(k=FAKE + (1 << 44), v=FAKE + (1 << 45))
+    assert lib.sa_kv_write(ctypes.byref(rows_args(s=seqs(**huge), **apart)), None) == UNSUPPORTED
+    assert lib.sa_kv_read(ctypes.byref(rows_args(s=seqs(**huge), **apart)), None) == UNSUPPORTED
+    args = attn_args(s=seqs(**huge), q=FAKE + (1 << 44), o=FAKE + (1 << 45), H=64)
+    assert lib.sa_kv_attention(ctypes.byref(args), None) == UNSUPPORTED
+    far = {n: FAKE + ((i + 1) << 44) for i, n in enumerate(("q", "k", "q_out", "k_out"))}
+    assert lib.sa_qk_norm_rope(ctypes.byref(rope_args(T=(1 << 31) - 1, **far)), None) == UNSUPPORTED
+
+
 def test_calls_with_nothing_to_do():
     lib = _lib.load()
     for none in (dict(B=0), dict(T=0), dict(max_rows=0)):
