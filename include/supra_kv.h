@@ -167,7 +167,7 @@ typedef struct sa_kv_attn_args {
   sa_kv_seqs seqs;
   int32_t H;
   int32_t causal;  /* 0 or 1 */
-  float scale;     /* finite */
+  float scale;     /* finite; magnitude below 2^127 */
   int32_t max_len; /* at least the longest seq_len, which shapes the launch (longer ones are still taken whole); 0: 32 * max_blocks */
   const void* q;
   void* o;

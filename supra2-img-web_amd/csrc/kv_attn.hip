@@ -1035,7 +1035,7 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   if (a->H <= 0 || a->H % a->cache.Hkv) return fail(SA_ERR_INVALID, "H = %d must be a positive multiple of Hkv = %d", a->H, a->cache.Hkv);
   if (a->H > (1 << 16)) return fail(SA_ERR_UNSUPPORTED, "%d heads (at most 65536)", a->H);
   if (a->causal != 0 && a->causal != 1) return fail(SA_ERR_INVALID, "causal must be 0 or 1 (got %d)", a->causal);
-  if (!isfinite(a->scale)) return fail(SA_ERR_INVALID, "scale must be finite");
+  if (!isfinite(a->scale * kLog2e)) return fail(SA_ERR_INVALID, "scale must be finite, and of magnitude below 2^127");
   if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
   *p = KvAttnParams{};
   *plan = KvAttnPlan{4, kRows, 0, 1, false, 0, 0};

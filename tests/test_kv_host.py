@@ -210,6 +210,13 @@ def test_refusals_of_attention(status, over):
 
 
 @no_device
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_scales_whose_log2_units_overflow_are_refused(scale):
+    """The kernels hold scores in log2 units: scale * log2(e) has to be a float32 number too."""
+    assert _lib.load().sa_kv_attention(ctypes.byref(attn_args(scale=scale)), None) == INVALID
+
+
+@no_device
 def test_refusals_of_the_workspace():
     """A call that splits its keys needs one: large enough, aligned, apart from everything else."""
     lib = _lib.load()
