@@ -1,18 +1,28 @@
 // Attention over the 8-bit key/value cache (include/supra_kv.h).
 //
-// One workgroup takes 32 rows (tokens x query heads of one key head: t * G + g) and a share of the sequence's pages;
-// its four waves take the pages in turn and their results are merged at the end. A page is 32 keys, the tile of a
-// 32x32x16 matrix instruction: S^T = K Q^T leaves a row's scores in the lanes l and l + 32 (register 4 g + r of half
-// h: key 8 g + 4 h + r), which is the operand order of O^T += V^T P^T, and the order V's codes have in the cache. So
-// neither K, V nor P changes lanes, and a page's K and V come as 16-byte loads of 1 KiB per wave.
+// A row is one token's query head: the rows t * G + g of one key head share its K and V, whatever token they are of. A
+// workgroup takes a group of such rows and a share of the sequence's pages. S^T = K Q^T leaves a row's scores in the
+// lanes that need them as the second operand of O^T += V^T P^T, and the cache's V codes lie in that order: neither K, V
+// nor P changes lanes, and a page's K and V come as 16-byte loads of 1 KiB per wave. The maximum and sum of the softmax
+// run along in float32. Two kernels, chosen by the rows of a sequence and key head (kv_attn_plan):
+//
+// kv_attn_split_kernel, up to 64 rows: 16 or 32 rows to a workgroup, whose four or eight waves take the pages in turn and
+//   are merged at the end. Bound by the cache's bytes: 64 sequences of 333 .. 8191 tokens, 8 key heads x 128, 117 us or
+//   4.8 TB/s of codes (a copy of 4 GiB reaches 4.6); 2 of 131000 tokens at 4 x 128, 54 us with their merge. Where there
+//   are too few workgroups the pages are split over several, whose records kv_attn_merge_kernel joins.
+// kv_attn_rows_kernel, more rows: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
+//   of the matrix and vector instructions together: 4 x 2048 rows over 4096 keys, 32 heads x 128, bfloat16, 560 us or
+//   0.98 PFLOP/s, with vector instructions in 59% of the cycles and matrix ones in 40% (an 8192^3 product of the
+//   library: 1.2). Short calls of it are bound by q and o instead: 64 x 256 rows over up to 128 keys, 9 heads x 64,
+//   float32, 25 us for 75 MB.
 //
 // Numbers. K and V codes are exact in float16 (v_cvt_scalef32_pk_f16_fp8), V's with its page's scale relative to the
 // largest one so far (2^m_v; a growing one rescales the sums like the running maximum). Q is brought to float16 by a
 // power of two of each row, its largest magnitude in [2^14, 2^15): float16 and bfloat16 rows in one term, exactly down
-// to 2^-28 of the row's largest element; float32 rows in two terms, 22 bits of each element. The probabilities, at
-// 2^kPBias for the running maximum, are one float16 term (11 bits: half a step of it is a sixteenth of a bfloat16
-// output's, and half a float16 one's, before the sum averages them) or two for float32 rows. Sums, maxima and products
-// are float32.
+// to 2^-28 of the row's largest element; float32 rows in two terms, 22 bits of each element. (The kernel of many rows
+// takes bfloat16 rows in two e4m3 terms: QCodes.) The probabilities, at 2^kPBias for the running maximum, are one
+// float16 term (11 bits: half a step of it is a sixteenth of a bfloat16 output's, and half a float16 one's, before the
+// sum averages them) or two for float32 rows. Sums, maxima and products are float32.
 //
 // V relative to the largest scale: codes times 2^(e - m_v + 6) stay exact for pages down to 2^-21 of the largest
 // page of the head, and below that are off by at most 2^-40 of its largest value.
@@ -914,7 +924,7 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
 }
 
 // The records of a row's splits into the row, a workgroup for each row: the weights of its splits in LDS, then D/4
-// threads to a record and 1024 / D records at a time, joined through LDS.
+// threads to a record and 1024 / D records at a time, joined through LDS. Latency: 3.9 us of 11 for 32 rows x 4 splits.
 constexpr int kMaxSplits = 512;
 
 template <typename T, int D>
@@ -979,11 +989,17 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
-  // Few rows, a quarter of the CUs to all of them with a workgroup each: eight waves to a workgroup, and the keys
-  // split (which costs the second launch) from 64 pages on. Against four waves and splits of eight pages: 16
-  // sequences of 2000 tokens at 8 key heads x 128 18.4 us (20.9), 32 of them 31.5 (35.5), 16 of 500 11.4 (13.0). With
-  // fewer workgroups the splits are quicker: one sequence of 2047 tokens 15.0 us in eight waves, 11.2 split.
-  p.waves = !p.many && base >= kCUs / 4 && base <= kCUs ? 8 : 4;
+  // Few rows and more than eight pages: eight waves to a workgroup instead of four and splits of eight pages (which cost
+  // the second launch):
+  // - with a workgroup for at least a quarter of the CUs; their keys are split from 64 pages on. 16 sequences of 2000
+  //   tokens at 8 key heads x 128 18.4 us (20.9), 32 of them 31.5 (35.5), 16 of 500 11.4 (13.0); at 8 x 256 in float16 32
+  //   of 777 27.2 (33.6), 16 of 2000 41.0 (38.0), 32 of 2000 56.5 (60.7);
+  // - with fewer, while eight waves have few pages each: one sequence of 777 tokens at 8 x 128 9.6 us (11.2), 1000 10.2
+  //   (11.2), 1400 11.3 (11.1), 2000 13.5 (11.4); at 8 x 64 in float32, 1400 8.9 (10.4), 2000 10.6 (10.7); at 8 x 256
+  //   777 14.8 (13.2).
+  // Eight pages or fewer are done in four waves, without a split: 16 of 200 tokens at 8 x 256 11.2 us (12.7).
+  const bool wide = base >= kCUs / 4 || (a->cache.D <= 128 && blocks * a->cache.D <= 4096);
+  p.waves = !p.many && base <= kCUs && blocks > 8 && wide ? 8 : 4;
   int64_t splits = 1;
   if (p.waves == 4) {
     splits = (2 * kCUs + base - 1) / base;

@@ -2,15 +2,19 @@
 //
 // A page and head of K or V is one tile of 32 tokens x D codes with one exponent byte. Both kernels give a wave one
 // such tile: what it reads and writes is contiguous on the cache's side and whole rows' heads on the other, and
-// the page's scale is a reduction inside the wave. Which sequence, page and head that is follows from the
-// workgroup index and the device's own lengths; waves beyond a sequence's pages end at once.
+// the page's scale is a reduction inside the wave, so the rows are read once and stay in registers until it is known.
+// Which sequence, page and head that is follows from the workgroup index and the device's own lengths; waves beyond a
+// sequence's pages end at once. Two waves to a workgroup: four hold its registers until the slowest is done (33 us
+// against 36 for the prompts below, with the earlier codes of a page loaded only by waves that must keep some).
 //
-// Quantising: with e the page's exponent byte, code = e4m3(x * 2^(127 - e)). The factor is a power of two, so the
-// product is exact (or below every e4m3 value's half), and v_cvt_pk_fp8_f32 rounds it once, to nearest even. A
+// Quantising: with e the page's exponent byte, code = e4m3(x * 2^(127 - e)). v_cvt_scalef32_pk_fp8_* takes the
+// factor as a power of two and rounds once, to nearest even (46 us with a multiplication and a conversion each). A
 // page that holds earlier tokens keeps max(its exponent, the new tokens'): codes that must move to a larger scale
-// are decoded, multiplied by a power of two and rounded the same way.
+// are decoded, which is exact, and rounded at the new one the same way.
 //
-// Bound: HBM traffic (rows in, a quarter to a half of it out).
+// Bound: HBM traffic. Written and read back: 5 prompts of 1 .. 4095 tokens, 8 heads x 128, bfloat16, 33 us for 129 MB,
+// 3.9 TB/s (a copy of 4 GiB reaches 4.6). One new token of each of 64 sequences, 13 us for both launches: latency, a page
+// rewritten for a token.
 
 #include <hip/hip_runtime.h>
 

@@ -326,7 +326,11 @@ def test_attention_splits_and_their_merge(dev):
     assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, max_len=500) == 1  # eight waves a workgroup
     assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, extra=70) > 1
     assert check_attention(dev, rng, [3] * 20, [n + 3 for n in lens], 32, 4, 64, "F32", True, extra=70) > 1  # 32 rows
-    assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 128, "BF16", True, max_len=500) > 1  # four waves
+    assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 128, "BF16", True, max_len=500) == 1  # few pages in eight waves
+    assert check_attention(dev, rng, [1] * 10, [n + 900 for n in lens[:10]], 4, 4, 128, "BF16", True, max_len=1400) > 1  # four waves
+    assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 256, "BF16", True, max_len=500) > 1  # wide heads
+    assert check_attention(dev, rng, [5, 1], [300, 290], 8, 2, 64, "F32", True, max_len=300) == 1  # 32 rows in eight waves
+    assert check_attention(dev, rng, [1, 1], [256, 257], 2, 1, 128, "F16", True, max_len=257) == 1  # nine pages
     assert check_attention(dev, rng, [100], [600], 2, 1, 64, "F16", True) > 1  # 128 rows each
 
 
