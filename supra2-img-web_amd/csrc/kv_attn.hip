@@ -11,8 +11,8 @@
 //   4.8 TB/s of codes (a copy of 4 GiB reaches 4.6); 2 of 131000 tokens at 4 x 128, 54 us with their merge. Where there
 //   are too few workgroups the pages are split over several, whose records kv_attn_merge_kernel joins.
 // kv_attn_rows_kernel, more rows: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
-//   of the matrix and vector instructions together: 4 x 2048 rows over 4096 keys, 32 heads x 128, bfloat16, 560 us or
-//   0.98 PFLOP/s, with vector instructions in 59% of the cycles and matrix ones in 40% (an 8192^3 product of the
+//   of the matrix and vector instructions together: 4 x 2048 rows over 4096 keys, 32 heads x 128, bfloat16, 565 us or
+//   0.97 PFLOP/s, with vector instructions in 59% of the cycles and matrix ones in 40% (an 8192^3 product of the
 //   library: 1.2). Short calls of it are bound by q and o instead: 64 x 256 rows over up to 128 keys, 9 heads x 64,
 //   float32, 25 us for 75 MB.
 //
@@ -762,14 +762,16 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void kv_attn_split_kernel
   }
 }
 
-// ---- many rows: 128 of them to a workgroup, 32 to a wave, and the pages of all through LDS. A stage is kStage pages,
-// loaded to registers while the one before is worked on and then left in one of two LDS buffers, so a stage costs
-// one barrier; in LDS a lane's 16 bytes of a KiB lie at 16 * lane, which neither its write nor its read conflicts on.
+// ---- many rows: 128 of them to a workgroup, 32 to a wave, and the pages of all through LDS. A stage is a page (two of
+// 64 channels), loaded to registers while the one before is worked on and then left in one of two LDS buffers, so a
+// stage costs one barrier; in LDS a lane's 16 bytes of a KiB lie at 16 * lane, which neither its write nor its read
+// conflicts on. Stages of one page against two: 4 x 1024 rows over 4096 keys at 16 heads x 256 334 us (365), 4 x 2048 at
+// 32 x 128 567 (573); at 64 channels prompts of 1024 .. 2048 rows 137 (130).
 constexpr int kRowWaves = 4;
-constexpr int kStage = 2;
 
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
+  constexpr int kStage = D <= 64 ? 2 : 1;
   constexpr int C = D / 32, ITEMS = kStage * 2 * C, MINE = ITEMS / kRowWaves;  // KiB of a stage, and a wave's
   static_assert(ITEMS % kRowWaves == 0, "whole KiB per wave");
   constexpr int BYTES = 2 * ITEMS * 1024 > kRowWaves * kRowsLds ? 2 * ITEMS * 1024 : kRowWaves * kRowsLds;
