@@ -120,11 +120,12 @@ __device__ __forceinline__ bool kv_work(const KvAttnParams& a, int rows, int gro
 }
 
 // Factor that brings a row whose largest magnitude has the bits m to float16: 2^(14 - its exponent), with the scale's
-// sign; the row is 2^exponent times that. An infinity or NaN in it gives NaN scores, as in float32.
+// sign; the row is 2^exponent times that. A row with an infinity or NaN has infinite or NaN scores alone, and so NaN
+// where it attends to anything, also where they are all -infinity, which the running maximum would pass over: NaN.
 __device__ __forceinline__ float q_factor(const KvAttnParams& a, uint32_t m, int& exponent) {
   const int f = min(127 + 14 + 127 - (int)(m >> 23), 253);
   exponent = 127 - f;
-  return copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
+  return m >= 0x7f800000u ? NAN : copysignf(__uint_as_float((uint32_t)f << 23), a.scale_log2);
 }
 
 // Q's operand for one 32-row group. float16 terms, one for float16 rows and two for float32: lane (row = lane & 31, half) has elements 32 c +

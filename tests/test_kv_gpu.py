@@ -398,6 +398,33 @@ def test_attention_queries_of_every_size(dev, dtype):
     cached.release()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_infinite_scores(dev, dtype, D, sign):
+    """An infinity in a row makes each of its scores infinite, here all of one sign: the row is NaN, whichever it is (the
+    differences of equal infinities), where it attends to anything; the other rows are as ever."""
+    rng = np.random.default_rng(19)
+    for rows, n in ((1, 40), (3, 40), (20, 40), (90, 40), (1, 2500)):
+        cache, table = filled(rng, dev, [n], 1, D)
+        cache.codes[0, :, :, :, 0] = 0xB8  # K's first element: -1, in every place
+        cached = Cached(dev, cache)
+        x = rng.standard_normal((rows, 2 * D))
+        x[rows // 2, D] = sign * np.inf
+        q = ok.to_type(x, dtype)
+        for causal in (False, True):
+            seqs = Sequences(dev, ok.Seqs([n], table, rows, rows))
+            got, ro, _ = attend(dev, cached, seqs, q, 2, dtype, 0.125, causal)
+            qv = ok.values(q, dtype).reshape(rows, 2, D)
+            with np.errstate(invalid="ignore"):
+                o, size, reach, count, _ = cache.attention(seqs.oracle, qv, 0.125, causal)
+            o[(~np.isfinite(qv).all(-1)) & (count > 0)[:, None]] = np.nan
+            near(got, o, ok.attention_tolerance(o, size, reach, count, D, dtype), f"rows {rows} of {n} causal {causal}")
+            ro.release()
+            seqs.release()
+        cached.release()
+
+
 def test_without_pages_and_with_shared_ones(dev):
     """No column in the block table: rows of zeros. One page in the tables of 70000 sequences: the same row for each."""
     rng = np.random.default_rng(17)
