@@ -59,6 +59,8 @@ struct KvAttnParams {
   int groups;     // row groups of a sequence (of max_rows)
   int splits;
   int aligned_q, aligned_o;  // rows of 16-byte aligned heads
+  int ordered;    // many rows: the workgroups with most pages first
+  int len_blocks; // pages of the longest sequence, as the caller has it
 };
 
 template <typename T>
@@ -770,6 +772,57 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void kv_attn_split_kernel
 // 32 x 128 567 (573); at 64 channels prompts of 1024 .. 2048 rows 137 (130).
 constexpr int kRowWaves = 4;
 
+// Workgroup number `rank` of one key head when those of all sequences (at most 64, one to a lane) stand in the order
+// of their pages, most first: its sequence and its place there; false past the last. Ragged prompts end with their
+// short workgroups instead of whichever come last: 8 of up to 2048 rows over 4096 keys, 32 heads on 8 x 128, 527 us ->
+// 332, 64 of up to 512 over 2048 459 -> 412, 16 of up to 1024 at 8 x 64 in float32 42.5 -> 39; 64 x 256 rows over
+// contexts of up to 512 keys, 9 x 64 in float32, 49 -> 43.5. Equal sequences pay for it: 4 x 2048 rows over 4096 keys
+// 437 -> 441, and short ones: 64 prompts of up to 512 tokens at 8 x 64 29 -> 30.3. So from 16 pages on, 32 where causal.
+// Pages grow with the place in a sequence, so the workgroups of a sequence with at least c pages are its last ones,
+// and their number follows from c alone; the c of this rank is searched for by halves.
+__device__ __forceinline__ bool longest_first(const KvAttnParams& a, int rank, int* b, int* place) {
+  constexpr int ROWS = kRows * kRowWaves;
+  const int lane = threadIdx.x & 63, lanes = min(a.s.B, 64);
+  KvSeq q{0, 0, 0, 0};
+  if (lane < lanes) q = kv_seq(a.s, lane);
+  const int all = (q.rows * a.G + ROWS - 1) / ROWS;
+  const auto sum = [](int x) {  // over the rows of 16 lanes by rotations (0x120 + n: by n lanes), then of the four rows
+    x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);
+    return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48);
+  };
+  const auto at_least = [&](int c) {  // of this lane's workgroups
+    const int keys = kKvBlock * (c - 1);  // with more of them: those from token t on
+    if (c == 0) return all;
+    if (q.len <= keys) return 0;
+    const int t = a.causal ? keys - q.first : 0;
+    return t >= q.rows ? 0 : t <= 0 ? all : all - t * a.G / ROWS;
+  };
+  if (rank >= sum(all)) return false;
+  int c = 0, end = a.s.max_blocks + 1;  // sum(at_least(c)) > rank >= sum(at_least(end))
+  if (a.len_blocks + 1 < end && sum(at_least(a.len_blocks + 1)) <= rank) end = a.len_blocks + 1;
+  while (end - c > 1) {
+    const int mid = (c + end) / 2;
+    if (sum(at_least(mid)) > rank) c = mid;
+    else end = mid;
+  }
+  const int more = at_least(c + 1), mine = at_least(c) - more;  // with more than c pages; with c
+  int before = mine;  // those of the lanes before, then without this one's
+  for (int m = 1; m < lanes; m <<= 1) {
+    const int x = __shfl_up(before, m);
+    if (lane >= m) before += x;
+  }
+  before -= mine;
+  const int here = rank - sum(more) - before;  // within this lane's, if it is one of them
+  const uint64_t found = __ballot(here >= 0 && here < mine);
+  const int from = __builtin_ctzll(found);
+  *b = from;
+  *place = __builtin_amdgcn_readlane(all - more - 1 - here, from);
+  return true;
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
   constexpr int kStage = D <= 64 ? 2 : 1;
@@ -783,12 +836,12 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
   int id = blockIdx.x;
   const int split = id % a.splits;
   id /= a.splits;
-  const int wide = (a.groups + kRowWaves - 1) / kRowWaves;  // workgroups of a sequence's rows
-  const int heads = a.s.B * a.c.Hkv;
-  const int block4 = wide - 1 - id / heads;
-  id %= heads;
+  const int hk = id % a.c.Hkv;
+  id /= a.c.Hkv;
+  int b = id % a.s.B, block4 = (a.groups + kRowWaves - 1) / kRowWaves - 1 - id / a.s.B;  // of a sequence's rows, the last first
+  if (a.ordered && !longest_first(a, id, &b, &block4)) return;
   Work all, w;
-  if (!kv_work(a, kRows, block4 * kRowWaves, id % a.c.Hkv, id / a.c.Hkv, &all)) return;
+  if (!kv_work(a, kRows, block4 * kRowWaves, hk, b, &all)) return;
   w = all;
   // pages of the workgroup: those of its last rows
   {
@@ -978,6 +1031,8 @@ struct KvAttnPlan {
   int waves;                       // of a workgroup
   int group_rows, groups, splits;  // of a row group; row groups of a sequence and key head; workgroups that share their keys
   bool many;                       // the kernel of many rows
+  bool ordered;                    // its workgroups by their pages
+  int64_t blocks;                  // pages of the longest sequence, as the caller has it
   int64_t workgroups, ws_bytes;
 };
 
@@ -1013,6 +1068,8 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   }
   if (splits < 1) splits = 1;
   p.splits = (int)splits;
+  p.blocks = blocks;
+  p.ordered = p.many && p.groups > kRowWaves && a->seqs.B > 1 && a->seqs.B <= 64 && blocks >= (a->causal ? 32 : 16);  // longest_first
   p.workgroups = base * splits;
   p.ws_bytes = splits > 1 ? (int64_t)a->seqs.B * a->cache.Hkv * p.groups * splits * record_floats(p.group_rows, a->cache.D) * 4 : 0;
   return p;
@@ -1057,7 +1114,7 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   if (!isfinite(a->scale * kLog2e)) return fail(SA_ERR_INVALID, "scale must be finite, and of magnitude below 2^127");
   if (a->max_len < 0) return fail(SA_ERR_INVALID, "max_len must be >= 0");
   *p = KvAttnParams{};
-  *plan = KvAttnPlan{4, kRows, 0, 1, false, 0, 0};
+  *plan = KvAttnPlan{4, kRows, 0, 1, false, false, 0, 0, 0};
   if (kv_nothing(a->seqs)) return SA_OK;
   const int size = kv_type_bytes(a->dtype);
   const int64_t width = (int64_t)a->H * a->cache.D;
@@ -1085,6 +1142,8 @@ int resolve_kv_attn(const sa_kv_attn_args* a, KvAttnParams* p, KvAttnPlan* plan)
   p->causal = a->causal;
   p->groups = plan->groups;
   p->splits = plan->splits;
+  p->ordered = plan->ordered;
+  p->len_blocks = (int)plan->blocks;
   p->aligned_q = (((uintptr_t)q.lo | (uintptr_t)q.ld) & 15) == 0;
   p->aligned_o = (((uintptr_t)o.lo | (uintptr_t)o.ld) & 15) == 0;
   return SA_OK;

@@ -334,6 +334,23 @@ def test_attention_splits_and_their_merge(dev):
     assert check_attention(dev, rng, [100], [600], 2, 1, 64, "F16", True) > 1  # 128 rows each
 
 
+@pytest.mark.parametrize("B", [2, 3, 33, 64, 65])
+@pytest.mark.parametrize("G,causal", [(1, True), (3, True), (2, False)])
+def test_attention_of_ragged_prompts(dev, B, G, causal):
+    """Prompts of many lengths in one call, whose workgroups are taken by their pages (up to 64 sequences): without rows,
+    of one, all of a sequence's tokens, more rows than tokens, no tokens, the same length twice, longer than max_len says."""
+    rng = np.random.default_rng(23 + B)
+    rows = [int(r) for r in rng.integers(0, 60 if B > 3 else 400, B)]
+    lens = [int(n) for n in rng.integers(1, 1300, B)]
+    rows[0], lens[0], rows[1], lens[1] = 300, 1290, 260, 260
+    if B > 6:
+        rows[2], rows[3], rows[4], lens[4], rows[5], lens[5], lens[6] = 0, 1, 45, 20, 33, 0, lens[7]
+    for dtype, D, max_len in (("BF16", 64, 0), ("F16", 128, 1100), ("F32", 64, 1024)):
+        check_attention(dev, rng, rows, lens, G, 1, D, dtype, causal, max_len=max_len)
+    if B == 3:
+        check_attention(dev, rng, rows, lens, 2 * G, 2, 256, "BF16", causal, extra=40)  # the keys split too
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_forms(dev, dtype):
     """Uniform rows without row_start; odd offsets and strides of q and o; large and tiny queries; scales far apart."""
