@@ -110,7 +110,7 @@ int64_t sa_kv_cache_bytes(int32_t pages, int32_t Hkv, int32_t D);
  * 0 .. max_rows and within the T rows, and a page id outside 0 .. pages-1 is a page that holds nothing (writes
  * to it are dropped, reads give zeros, attention passes its tokens over). Rows of the outputs that belong to no
  * sequence are left as they were. Pages may be shared by sequences that only read them; two sequences of one
- * write call must not write to the same page, and no two sequences of a call have a row in common (what such calls
+ * write call, or two places of one sequence, must not write to the same page, and no two sequences of a call have a row in common (what such calls
  * leave is some mixture of both). A call's launch is shaped by the bounds: a batch of prompts and single tokens is
  * quicker as two calls, one with max_rows 1.
  */

@@ -327,8 +327,8 @@ __device__ __forceinline__ void step(const Q& q, State<D>& st, const LoadK& k, c
                                      int lane, int limit) {
   constexpr int NT = kTerms<T>;
   // Where registers allow, the whole page is on its way before the first product (the compiler would fetch V's part
-  // after the exponentials: 630 us against 619 for 4 x 2048 rows over 4096 keys at 32 heads x 128).
-  constexpr bool EARLY = D <= 128;
+  // after the exponentials: 571 us against 565 for 4 x 2048 rows over 4096 keys at 32 heads x 128).
+  constexpr bool EARLY = D == 128 || (D == 64 && sizeof(T) == 4);
   u32x4 kr[D / 32], vr[D / 32];
   if constexpr (EARLY) {
 #pragma unroll
@@ -765,11 +765,12 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void kv_attn_split_kernel
   }
 }
 
-// ---- many rows: 128 of them to a workgroup, 32 to a wave, and the pages of all through LDS. A stage is a page (two of
-// 64 channels), loaded to registers while the one before is worked on and then left in one of two LDS buffers, so a
-// stage costs one barrier; in LDS a lane's 16 bytes of a KiB lie at 16 * lane, which neither its write nor its read
-// conflicts on. Stages of one page against two: 4 x 1024 rows over 4096 keys at 16 heads x 256 334 us (365), 4 x 2048 at
-// 32 x 128 567 (573); at 64 channels prompts of 1024 .. 2048 rows 137 (130).
+// ---- many rows: 128 of them to a workgroup, 32 to a wave, and the pages of all through LDS. A page is loaded to
+// registers while the one before is worked on and then left in one of two LDS buffers, so it costs one barrier (two pages
+// to a barrier: 4 x 1024 rows over 4096 keys at 16 heads x 256 365 us against 334, 4 x 2048 at 32 x 128 573 against 567);
+// in LDS a lane's 16 bytes of a KiB lie at 16 * lane, which neither its write nor its read conflicts on. Four waves to a
+// SIMD for 16-bit rows of 64 channels (4 x 2048 rows over 4096 keys at 16 heads 178 us, in three 200), three for float32
+// ones, two and one for the wider heads: what the registers allow without spills.
 constexpr int kRowWaves = 4;
 
 // Workgroup number `rank` of one key head when those of all sequences (at most 64, one to a lane) stand in the order
@@ -824,12 +825,11 @@ __device__ __forceinline__ bool longest_first(const KvAttnParams& a, int rank, i
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
-  constexpr int kStage = D <= 64 ? 2 : 1;
-  constexpr int C = D / 32, ITEMS = kStage * 2 * C, MINE = ITEMS / kRowWaves;  // KiB of a stage, and a wave's
+__global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? (sizeof(T) == 2 ? 4 : 3) : D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnParams a) {
+  constexpr int C = D / 32, ITEMS = 2 * C, MINE = ITEMS / kRowWaves;  // KiB of a page, and a wave's
   static_assert(ITEMS % kRowWaves == 0, "whole KiB per wave");
   constexpr int BYTES = 2 * ITEMS * 1024 > kRowWaves * kRowsLds ? 2 * ITEMS * 1024 : kRowWaves * kRowsLds;
-  __shared__ __attribute__((aligned(16))) char shared[BYTES];  // the stages; before and after them, the waves' rows
+  __shared__ __attribute__((aligned(16))) char shared[BYTES];  // the pages; before and after them, the waves' rows
   u32x4(&tiles)[2][ITEMS][64] = *reinterpret_cast<u32x4(*)[2][ITEMS][64]>(shared);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -867,31 +867,22 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
   const int32_t* table = a.s.block_table + (int64_t)w.b * a.s.max_blocks;
   const int place = (lane & 31) * 32 + (lane >> 5) * 16;
   u32x4 part[MINE];
-  int pages[kStage], ke[kStage], ve[kStage];  // of the stage being loaded; a page that holds nothing: -1
-  int32_t ids[kStage];  // of the stage after that: a page's loads wait for its id, so it comes a stage earlier
-  const auto look = [&](int blk) {
-#pragma unroll
-    for (int p = 0; p < kStage; ++p) ids[p] = blk + p < hi_block ? table[blk + p] : -1;
-  };
+  int page, ke, ve;  // of the page being loaded; one that holds nothing: -1
+  int32_t id_next;   // of the page after that: a page's loads wait for its id, so it comes a page earlier
+  const auto look = [&](int blk) { id_next = blk < hi_block ? table[blk] : -1; };
   const auto fetch = [&](int blk) {
-#pragma unroll
-    for (int p = 0; p < kStage; ++p) {
-      pages[p] = kv_page_ok(ids[p], a.c.pages) ? ids[p] : -1;
-      const int64_t at = (int64_t)max(pages[p], 0) * a.c.Hkv + w.hk;
-      ke[p] = a.c.k_scale[at];
-      ve[p] = a.c.v_scale[at];
-    }
+    page = kv_page_ok(id_next, a.c.pages) ? id_next : -1;
+    const int64_t at = (int64_t)max(page, 0) * a.c.Hkv + w.hk;
+    ke = a.c.k_scale[at];
+    ve = a.c.v_scale[at];
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-      const int item = wave + kRowWaves * j, p = item / (2 * C), c = item % C;
-      const bool is_v = item / C & 1;
-      int page = pages[0];
-#pragma unroll
-      for (int i = 1; i < kStage; ++i) page = p == i ? pages[i] : page;
+      const int item = wave + kRowWaves * j, c = item % C;
+      const bool is_v = item / C & 1;  // (as a comparison of item with C it compiles to 395 us for 335 at 4 x 1024 rows, 16 heads x 256)
       const uint8_t* base = (is_v ? a.c.v : a.c.k) + kv_tile(max(page, 0), a.c.Hkv, w.hk, D);
       part[j] = *reinterpret_cast<const u32x4*>(base + c * 1024 + place);
     }
-    look(blk + kStage);
+    look(blk + 1);
   };
   const auto leave = [&](int buf) {
 #pragma unroll
@@ -904,37 +895,31 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? 3 : D <= 128 ? 2 : 1) voi
     __syncthreads();  // every wave has its rows
     leave(0);
   }
-  // Stages that every row of the workgroup attends to as a whole, then the others.
+  // Pages that every row of the workgroup attends to as a whole, then the others.
   const float scale = fabsf(a.scale_log2);
   int buf = 0;
-  const auto stages = [&](int begin, int end, auto masked) {
+  const auto steps = [&](int begin, int end, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
-    for (int blk = begin; blk < end; blk += kStage, buf ^= 1) {
-      int now[kStage], kn[kStage], vn[kStage];
-#pragma unroll
-      for (int p = 0; p < kStage; ++p) now[p] = pages[p], kn[p] = ke[p], vn[p] = ve[p];
+    for (int blk = begin; blk < end; ++blk, buf ^= 1) {
+      const int now = page, kn = ke, vn = ve;
       __syncthreads();
-      const bool more = blk + kStage < hi_block;
-      if (more) fetch(blk + kStage);
-      if (on) {
-#pragma unroll
-        for (int p = 0; p < kStage; ++p) {
-          if (now[p] < 0 || (MASKED && blk + p >= w.blocks)) continue;
-          const auto k = [&](int c) { return tiles[buf][p * 2 * C + c][lane]; };
-          const auto v = [&](int c) { return tiles[buf][p * 2 * C + C + c][lane]; };
-          const int kk = __builtin_amdgcn_readfirstlane(kn[p]), vv = __builtin_amdgcn_readfirstlane(vn[p]);
-          step<T, D, MASKED>(q, st, k, v, kk, vv, scale, lane, limit - (blk + p) * kKvBlock);
-        }
+      const bool more = blk + 1 < hi_block;
+      if (more) fetch(blk + 1);
+      if (on && now >= 0 && !(MASKED && blk >= w.blocks)) {
+        const auto k = [&](int c) { return tiles[buf][c][lane]; };
+        const auto v = [&](int c) { return tiles[buf][C + c][lane]; };
+        const int kk = __builtin_amdgcn_readfirstlane(kn), vv = __builtin_amdgcn_readfirstlane(vn);
+        step<T, D, MASKED>(q, st, k, v, kk, vv, scale, lane, limit - blk * kKvBlock);
       }
       if (more) leave(buf ^ 1);
     }
   };
   int least = w.q.len;  // keys that the workgroup's first row attends to
   if (a.causal) least = max(0, min(least, w.q.first + block4 * kRowWaves * kRows / a.G + 1));
-  const int whole = max(lo_block, lo_block + (min(hi_block, least / kKvBlock) - lo_block) / kStage * kStage);
-  stages(lo_block, whole, std::false_type{});
-  stages(whole, hi_block, std::true_type{});
-  __syncthreads();  // the last stage is done with
+  const int whole = max(lo_block, min(hi_block, least / kKvBlock));
+  steps(lo_block, whole, std::false_type{});
+  steps(whole, hi_block, std::true_type{});
+  __syncthreads();  // the last page is done with
   if (!on) return;
 
   const float total = sum_with_partner(st.l);
