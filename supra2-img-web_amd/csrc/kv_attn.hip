@@ -4,13 +4,13 @@
 // workgroup takes a group of such rows and a share of the sequence's pages. S^T = K Q^T leaves a row's scores in the
 // lanes that need them as the second operand of O^T += V^T P^T, and the cache's V codes lie in that order: neither K, V
 // nor P changes lanes, and a page's K and V come as 16-byte loads of 1 KiB per wave. The maximum and sum of the softmax
-// run along in float32. Two kernels, chosen by the rows of a sequence and key head (kv_attn_plan):
+// run along in float32. Two kernels, chosen by the call's rows (kv_attn_plan):
 //
-// kv_attn_split_kernel, up to 64 rows: 16 or 32 rows to a workgroup, whose four or eight waves take the pages in turn and
+// kv_attn_split_kernel, few rows: 16 or 32 rows to a workgroup, whose four or eight waves take the pages in turn and
 //   are merged at the end. Bound by the cache's bytes: 64 sequences of 333 .. 8191 tokens, 8 key heads x 128, 117 us or
 //   4.8 TB/s of codes (a copy of 4 GiB reaches 4.6); 2 of 131000 tokens at 4 x 128, 54 us with their merge. Where there
 //   are too few workgroups the pages are split over several, whose records kv_attn_merge_kernel joins.
-// kv_attn_rows_kernel, more rows: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
+// kv_attn_rows_kernel, rows for more than 256 workgroups of 128: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
 //   of the matrix and vector instructions together: 4 x 2048 rows over 4096 keys, 32 heads x 128, bfloat16, 565 us or
 //   0.97 PFLOP/s, with vector instructions in 59% of the cycles and matrix ones in 40% (an 8192^3 product of the
 //   library: 1.2). Short calls of it are bound by q and o instead: 64 x 256 rows over up to 128 keys, 9 heads x 64,
@@ -645,20 +645,31 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void kv_attn_split_kernel
   __shared__ int lv[W];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int group = id % a.groups;
-  id /= a.groups;
+  // Splits first, so that long sequences spread over the XCDs; with several groups of rows, which read the same pages,
+  // key heads first and the groups next: where Hkv is a multiple of 8, a head's groups share an XCD's L2.
+  int id = blockIdx.x, split = 0, group = 0;
+  if (a.groups == 1) {
+    split = id % a.splits;
+    id /= a.splits;
+  }
+  const int hk = id % a.c.Hkv;
+  id /= a.c.Hkv;
+  if (a.groups > 1) {
+    group = id % a.groups;
+    id /= a.groups;
+    split = id % a.splits;
+    id /= a.splits;
+  }
+  const int b = id;
   // With all pages of a sequence in one workgroup, the first ones' ids need not wait for its length.
-  const int32_t* table = a.s.block_table + (int64_t)(id / a.c.Hkv) * a.s.max_blocks;
+  const int32_t* table = a.s.block_table + (int64_t)b * a.s.max_blocks;
   int32_t first = -1, next = -1;  // ids of the wave's first page, and of the page after the one being loaded
   if (a.splits == 1) {
     if (wave < a.s.max_blocks) first = table[wave];
     if (wave + W < a.s.max_blocks) next = table[wave + W];
   }
   Work w;
-  if (!kv_work(a, ROWS, group, id % a.c.Hkv, id / a.c.Hkv, &w)) return;
+  if (!kv_work(a, ROWS, group, hk, b, &w)) return;
   const int lo_block = (int)((int64_t)w.blocks * split / a.splits), hi_block = (int)((int64_t)w.blocks * (split + 1) / a.splits);
 
   int blk = lo_block + wave;
@@ -925,7 +936,8 @@ __global__ __launch_bounds__(64 * kRowWaves, D <= 64 ? (sizeof(T) == 2 ? 4 : 3) 
   const float total = sum_with_partner(st.l);
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int half = lane >> 5;
-  float* rec = a.splits > 1 ? a.ws + record_at(a, w.b, w.hk, w.row0 / kRows, split, kRows, D) : nullptr;
+  float* rec = nullptr;  // narrower heads come here only with more workgroups than their keys would be split for
+  if constexpr (D == 256) rec = a.splits > 1 ? a.ws + record_at(a, w.b, w.hk, w.row0 / kRows, split, kRows, D) : nullptr;
   if (rec && half == 0) rec[(int64_t)kRows * D + lane] = total == 0.f ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
   const int64_t at = row_place(a, w, row, a.ldo, D * (int)sizeof(T));
   // Through LDS, as Q came: E elements of a row in a lane, 16 bytes of a record or an output row.
@@ -1025,10 +1037,18 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   KvAttnPlan p;
   const int G = a->H / a->cache.Hkv;
   const int64_t rows = (int64_t)a->seqs.max_rows * G;
-  p.many = rows > 64;
-  p.group_rows = p.many ? kRows : rows <= 16 || a->cache.D == 256 ? 16 : 32;
+  const int64_t heads = (int64_t)a->seqs.B * a->cache.Hkv;
+  // The kernel of many rows where it has work for all CUs, from 128 rows on: its lone workgroups wait for each page in
+  // turn. In it / in groups of 32: one prompt of 1000 tokens at 32 heads on 8 x 64 60 us / 17, on 8 x 128 64 / 29, with
+  // 8000 keys 176 / 153; 16 of 64 over 1000 keys (128) 73 / 37, 32 of 64 52 / 87, 32 of 32 76 / 49. At 256 channels, whose
+  // groups are of 16 rows, from 64 on: 32 of 24 tokens over 1000 keys 103 / 122, of 16 89 / 86.
+  p.many = a->cache.D == 256 ? rows > 64 : rows > 128 && heads * ((rows + 127) / 128) > kCUs;
+  // Groups of 16 rows while a workgroup for each fits the CUs: 4 sequences of 12 rows x 8 heads over 2000 keys at 8 x 64
+  // in float32 12.0 us, in groups of 32 17.8; with more, 32 of 16 rows over 1000 keys (128) 43.5 / 28.6.
+  const bool narrow = a->cache.D == 256 || rows <= 16 || heads * ((rows + 15) / 16) <= kCUs;
+  p.group_rows = p.many ? kRows : narrow ? 16 : 32;
   p.groups = (int)((rows + p.group_rows - 1) / p.group_rows);
-  const int64_t base = (int64_t)a->seqs.B * a->cache.Hkv * (p.many ? (p.groups + kRowWaves - 1) / kRowWaves : p.groups);
+  const int64_t base = heads * (p.many ? (p.groups + kRowWaves - 1) / kRowWaves : p.groups);
   const int64_t cap = (int64_t)a->seqs.max_blocks * kKvBlock;
   const int64_t len = a->max_len > 0 && a->max_len < cap ? a->max_len : cap;
   const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
@@ -1043,12 +1063,18 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   // Eight pages or fewer are done in four waves, without a split: 16 of 200 tokens at 8 x 256 11.2 us (12.7).
   const bool wide = base >= kCUs / 4 || (a->cache.D <= 128 && blocks * a->cache.D <= 4096);
   p.waves = !p.many && base <= kCUs && blocks > 8 && wide ? 8 : 4;
+  // Splits fill two workgroups of four waves to a CU or one of eight, and no more (one too many is a round of its own:
+  // 20 sequences of 8000 tokens at 8 x 128 82 us for 65); few rows of one group in four waves are quicker past that.
+  // Many rows pay for splits with a record of each (1200 rows x 8 heads over 1000 keys at 64 channels, two splits 28.7
+  // us, one 13), worth it only where the last round would be nearly empty: 12 x 80 tokens over 8000 keys at 32 heads on
+  // 8 x 256 807 us, in one 986.
   int64_t splits = 1;
   if (p.waves == 4) {
-    splits = (2 * kCUs + base - 1) / base;
+    splits = (2 * kCUs + (p.groups > 1 ? 0 : base - 1)) / base;
+    if (p.many && base > kCUs && base <= kCUs + kCUs / 4 && a->cache.D == 256 && blocks >= 128) splits = 2;
     if (splits > (blocks + 7) / 8) splits = (blocks + 7) / 8;
   } else if (blocks > 64) {
-    splits = (kCUs + base - 1) / base;
+    splits = kCUs / base;
     if (splits > (blocks + 31) / 32) splits = (blocks + 31) / 32;
   }
   if (splits < 1) splits = 1;

@@ -325,13 +325,19 @@ def test_attention_splits_and_their_merge(dev):
     lens = [int(n) for n in rng.integers(1, 500, 20)]
     assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, max_len=500) == 1  # eight waves a workgroup
     assert check_attention(dev, rng, [1] * 20, lens, 8, 4, 64, "F16", True, extra=70) > 1
-    assert check_attention(dev, rng, [3] * 20, [n + 3 for n in lens], 32, 4, 64, "F32", True, extra=70) > 1  # 32 rows
+    assert check_attention(dev, rng, [3] * 20, [n + 3 for n in lens], 32, 4, 64, "F32", True, extra=70) == 1  # two groups of 16 rows
+    assert check_attention(dev, rng, [5] * 33, [n % 97 + 300 for n in range(33)], 32, 8, 64, "F32", True, max_len=400) > 1  # 32 rows
+    assert check_attention(dev, rng, [5] * 33, [n % 97 + 300 for n in range(33)], 32, 8, 128, "BF16", True, max_len=400) > 1
+    assert check_attention(dev, rng, [9] * 10, [n % 7 + 300 for n in range(10)], 32, 8, 128, "F16", True, max_len=400) == 1  # in eight waves
     assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 128, "BF16", True, max_len=500) == 1  # few pages in eight waves
     assert check_attention(dev, rng, [1] * 10, [n + 900 for n in lens[:10]], 4, 4, 128, "BF16", True, max_len=1400) > 1  # four waves
     assert check_attention(dev, rng, [1] * 10, lens[:10], 4, 4, 256, "BF16", True, max_len=500) > 1  # wide heads
-    assert check_attention(dev, rng, [5, 1], [300, 290], 8, 2, 64, "F32", True, max_len=300) == 1  # 32 rows in eight waves
+    assert check_attention(dev, rng, [5, 1], [300, 290], 8, 2, 64, "F32", True, max_len=300) == 1  # two groups in eight waves
     assert check_attention(dev, rng, [1, 1], [256, 257], 2, 1, 128, "F16", True, max_len=257) == 1  # nine pages
-    assert check_attention(dev, rng, [100], [600], 2, 1, 64, "F16", True) > 1  # 128 rows each
+    assert check_attention(dev, rng, [100], [600], 2, 1, 64, "F16", True) == 1
+    for dtype in TYPES:
+        assert check_attention(dev, rng, [100], [600], 2, 1, 256, dtype, True) > 1  # 128 rows each
+    assert check_attention(dev, rng, [35, 7, 34], [600, 3000, 41], 9, 1, 64, "BF16", True) > 1  # groups of 16 rows of three sequences
 
 
 @pytest.mark.parametrize("B", [2, 3, 33, 64, 65])
@@ -440,6 +446,46 @@ def test_attention_of_infinite_scores(dev, dtype, D, sign):
             ro.release()
             seqs.release()
         cached.release()
+
+
+class Wider(ok.Seqs):
+    """The same sequences under a bound of many more rows, which gives them to the kernel of 128 rows a workgroup."""
+
+    def __init__(self, seq_len, table, T, max_rows, row_start=None):
+        if row_start is None:
+            row_start = np.minimum(np.arange(len(seq_len) + 1) * max_rows, T)
+        super().__init__(seq_len, table, T, 40000, row_start)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_few_rows_as_of_many(dev, dtype, monkeypatch):
+    """The kernel of many rows on the rows, masks, NaN codes and queries that the other tests give the kernel of few."""
+    monkeypatch.setattr(ok, "Seqs", Wider)
+    for D in (64, 128, 256):
+        test_attention_tokens(dev, dtype, D, 7, 1)
+        for causal in (True, False):
+            test_attention_prompts(dev, dtype, D, causal)
+        test_attention_of_infinite_scores(dev, dtype, D, -1)
+    test_attention_forms(dev, dtype)
+    test_attention_nan_where_it_is_not_attended(dev, dtype)
+    test_attention_queries_of_every_size(dev, dtype)
+
+
+@pytest.mark.parametrize("B", [3, 64])
+@pytest.mark.parametrize("G,causal", [(1, True), (3, True), (2, False)])
+def test_attention_of_ragged_prompts_as_of_many(dev, B, G, causal, monkeypatch):
+    """Their workgroups by their pages: the order is the kernel of many rows' alone."""
+    monkeypatch.setattr(ok, "Seqs", Wider)
+    test_attention_of_ragged_prompts(dev, B, G, causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_many_rows_in_many_heads(dev, dtype, causal):
+    """More than 256 workgroups of 128 rows by the call's own sizes."""
+    rng = np.random.default_rng(29)
+    check_attention(dev, rng, [131], [200], 130, 130, 64, dtype, causal)
+    check_attention(dev, rng, [65, 2], [70, 40], 130, 65, 128, dtype, causal)
 
 
 def test_without_pages_and_with_shared_ones(dev):
