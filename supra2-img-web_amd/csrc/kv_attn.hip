@@ -10,7 +10,7 @@
 //   are merged at the end. Bound by the cache's bytes: 64 sequences of 333 .. 8191 tokens, 8 key heads x 128, 117 us or
 //   4.8 TB/s of codes (a copy of 4 GiB reaches 4.6); 2 of 131000 tokens at 4 x 128, 54 us with their merge. Where there
 //   are too few workgroups the pages are split over several, whose records kv_attn_merge_kernel joins.
-// kv_attn_rows_kernel, rows for more than 256 workgroups of 128: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
+// kv_attn_rows_kernel, rows for some 512 workgroups of 128 and more: 128 to a workgroup, 32 to a wave, the pages through LDS for all four. Bound by the issue
 //   of the matrix and vector instructions together: 4 x 2048 rows over 4096 keys, 32 heads x 128, bfloat16, 565 us or
 //   0.97 PFLOP/s, with vector instructions in 59% of the cycles and matrix ones in 40% (an 8192^3 product of the
 //   library: 1.2). Short calls of it are bound by q and o instead: 64 x 256 rows over up to 128 keys, 9 heads x 64,
@@ -1038,11 +1038,14 @@ KvAttnPlan kv_attn_plan(const sa_kv_attn_args* a) {
   const int G = a->H / a->cache.Hkv;
   const int64_t rows = (int64_t)a->seqs.max_rows * G;
   const int64_t heads = (int64_t)a->seqs.B * a->cache.Hkv;
-  // The kernel of many rows where it has work for all CUs, from 128 rows on: its lone workgroups wait for each page in
-  // turn. In it / in groups of 32: one prompt of 1000 tokens at 32 heads on 8 x 64 60 us / 17, on 8 x 128 64 / 29, with
-  // 8000 keys 176 / 153; 16 of 64 over 1000 keys (128) 73 / 37, 32 of 64 52 / 87, 32 of 32 76 / 49. At 256 channels, whose
-  // groups are of 16 rows, from 64 on: 32 of 24 tokens over 1000 keys 103 / 122, of 16 89 / 86.
-  p.many = a->cache.D == 256 ? rows > 64 : rows > 128 && heads * ((rows + 127) / 128) > kCUs;
+  // The kernel of many rows where it has two workgroups for each CU (one and a half of 16-bit rows of 128 channels), from
+  // 128 rows on: a lone workgroup waits for each page in turn. In it / in groups of 32: one prompt of 1000 tokens over 1000
+  // keys at 32 heads on 8 x 64 60 us / 17, on 8 x 128 64 / 29; 4 of 300 over 8000 (320 workgroups) at 8 x 64 200 / 126, on
+  // 8 x 128 247 / 198, one of 2000 (504) on 8 x 64 183 / 175, on 8 x 128 249 / 281, in float32 439 / 411; 32 of 64 over
+  // 1000 (512) on 8 x 128 52 / 87, 32 of 32 (rows of 128) 76 / 49. At 256 channels, whose groups are of 16 rows, from 64
+  // rows on: 32 of 24 tokens over 1000 keys 103 / 122, of 16 89 / 86.
+  const int64_t full = a->cache.D == 128 && a->dtype != SA_DT_F32 ? kCUs * 3 / 2 : 2 * kCUs;
+  p.many = a->cache.D == 256 ? rows > 64 : rows > 128 && heads * ((rows + 127) / 128) > full;
   // Groups of 16 rows while a workgroup for each fits the CUs: 4 sequences of 12 rows x 8 heads over 2000 keys at 8 x 64
   // in float32 12.0 us, in groups of 32 17.8; with more, 32 of 16 rows over 1000 keys (128) 43.5 / 28.6.
   const bool narrow = a->cache.D == 256 || rows <= 16 || heads * ((rows + 15) / 16) <= kCUs;

@@ -454,7 +454,7 @@ class Wider(ok.Seqs):
     def __init__(self, seq_len, table, T, max_rows, row_start=None):
         if row_start is None:
             row_start = np.minimum(np.arange(len(seq_len) + 1) * max_rows, T)
-        super().__init__(seq_len, table, T, 40000, row_start)
+        super().__init__(seq_len, table, T, 80000, row_start)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -482,10 +482,10 @@ def test_attention_of_ragged_prompts_as_of_many(dev, B, G, causal, monkeypatch):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_of_many_rows_in_many_heads(dev, dtype, causal):
-    """More than 256 workgroups of 128 rows by the call's own sizes."""
+    """More than 512 workgroups of 128 rows by the call's own sizes."""
     rng = np.random.default_rng(29)
-    check_attention(dev, rng, [131], [200], 130, 130, 64, dtype, causal)
-    check_attention(dev, rng, [65, 2], [70, 40], 130, 65, 128, dtype, causal)
+    check_attention(dev, rng, [131], [200], 257, 257, 64, dtype, causal)
+    check_attention(dev, rng, [65, 2], [70, 40], 258, 129, 128, dtype, causal)
 
 
 def test_without_pages_and_with_shared_ones(dev):
